@@ -440,6 +440,85 @@ int sbsa_repack_runs(const void* src_packed, void* dst_packed, int64_t packed_le
                      int32_t* posting, int64_t posting_width, int32_t* inverse, int64_t inverse_ld,
                      hipStream_t stream);
 
+/* ---- dense layers: rotary positions and an 8-bit key/value cache -----------------
+ * A hybrid model's dense layers, and the rotary step of its sparse ones.  These have
+ * no counterpart in the reference, whose host model rotates (the model's
+ * _project_qkv, semblo/vllm_plugin/qwen3_5_model.py:135) and whose dense layers are the engine's. */
+
+/* Rotary positions of a layer's queries and keys: for pair i of the first rotary_dim
+ * dimensions, (a, b) -> gain (a cos t - b sin t, b cos t + a sin t) at t = position x
+ * frequency i; the dimensions past rotary_dim are copied.  Pairs are (i, i + rotary_dim/2),
+ * or (2i, 2i+1) where interleaved.  q [tokens, num_q_heads, head_dim] bf16 at strides
+ * (q_st, q_sh), k likewise (num_kv_heads 0: no keys); the outputs may be the inputs
+ * themselves (same pointer and strides), and must not overlap them otherwise.
+ * turns [rotary_dim/2]: the frequency as a fraction of a turn per position, times 2^64,
+ * so that position x turns mod 2^64 is the angle at any position.  positions: int32 or
+ * int64 (pos_bytes 4 or 8), token t's on axis x at positions[x pos_axis_stride + t pos_stride];
+ * axes [rotary_dim/2] (bytes, or null: axis 0) is each pair's axis.  inverse: the
+ * rotation back, with 1 / gain.  rotary_dim even, head_dim up to 512. */
+int sbsa_rotary(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                int num_q_heads, const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st,
+                int64_t ko_sh, int num_kv_heads, const void* positions, int pos_bytes,
+                int64_t pos_axis_stride, int64_t pos_stride, int64_t tokens, int head_dim, int rotary_dim,
+                int interleaved, const uint64_t* turns, const uint8_t* axes, float gain, int inverse,
+                hipStream_t stream);
+
+#define SBSA_CACHE8_BLOCK 64    /* tokens of a block: one scale for its keys, one for its values */
+#define SBSA_CACHE8_E4M3 0      /* codes are OCP e4m3 numbers, the largest 448 */
+#define SBSA_CACHE8_INT8 1      /* codes are signed integers, the largest 127 */
+#define SBSA_CACHE8_MAX_BLOCKS 16384
+
+/* The cache of num_seqs sequences.  A block's place is table[seq, head, block], a permutation
+ * of 0 .. num_blocks-1 for each (seq, head); entries outside are read as the nearest place.
+ * A value is code x scale; a block that holds a value that is not finite has scale NaN.
+ * The codes behind a sequence's last token may hold anything. */
+typedef struct sbsa_cache8 {
+  void* codes_k;        /* [S, Hkv, N, 64, dim] bytes, 16-byte aligned            */
+  void* codes_v;        /* [S, Hkv, N, dim, 64] bytes, 16-byte aligned            */
+  float* scales;        /* [2, S, Hkv, N]: keys, values                           */
+  void* tail;           /* [2, S, Hkv, 64, dim] bf16: the rows of open_block      */
+  int32_t* table;       /* [S, Hkv, N]                                            */
+  float* weights;       /* [S, Hkv, N]: attention received by each block          */
+  int32_t* lengths;     /* [S, Hkv]: tokens held (the same for a sequence's heads) */
+  int32_t* open_block;  /* [S, Hkv]: the block whose rows tail holds, -1: none    */
+  int32_t* counters;    /* [S, Hkv], zero between calls                           */
+  int32_t* overflow;    /* [1]: set where rows found no room                      */
+  int32_t num_seqs, num_kv_heads, num_blocks, head_dim, format;
+} sbsa_cache8;
+
+/* New rows behind each sequence's tokens.  k, v [tokens, Hkv, dim] bf16; sequence s has rows
+ * offsets[s] .. offsets[s+1] (device int32 [S+1]; null: tokens / S rows each).  start (device int32
+ * [S], or null: the lengths): the rows go to start[s] onwards and the sequence ends behind them
+ * (start is at most the length; no rows: the sequence is cut there).  Each touched block is quantised
+ * whole from its bf16 rows: the new ones, and the earlier ones from tail, or from their codes where tail
+ * holds another block.  Rows past the room are dropped and overflow is set.  max_rows: a hint
+ * of the most rows of a sequence (any value gives the same result). */
+int sbsa_cache8_append(const sbsa_cache8* cache, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+                       int64_t v_st, int64_t v_sh, int64_t tokens, const int32_t* offsets,
+                       const int32_t* start, int64_t max_rows, hipStream_t stream);
+
+/* Attention of each sequence's newest tokens over its cache: row i of its n rows sees the first
+ * length - n + i + 1 tokens; a row that sees none gives 0 and -inf.  q, out [tokens, Hq, dim] bf16,
+ * lse [tokens, Hq] (natural; null only where accumulate is 0).  accumulate: weights[s, h, b] += the
+ * probabilities of block b's tokens over the rows and the head's query heads.  Rows of no sequence
+ * keep what out and lse held.  Hq / Hkv up to 16, dim 128 or 256.  max_rows: a hint as in append. */
+size_t sbsa_cache8_attend_workspace_bytes(const sbsa_cache8* cache, int num_q_heads, int64_t tokens,
+                                          int64_t max_rows, int ragged, int accumulate);
+int sbsa_cache8_attend(const sbsa_cache8* cache, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads,
+                       int64_t tokens, const int32_t* offsets, int64_t max_rows, float sm_scale, void* out,
+                       int64_t o_st, int64_t o_sh, float* lse, int accumulate, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/* The tables of a cache cut to at most keep blocks per (seq, head): the first sink blocks, the last
+ * recent ones and the heaviest of the others stay, in their order (of equal weights the
+ * earlier; a weight that is not above 0 counts as 0).  The places of the blocks that go follow those that stay, then
+ * the free ones; weights behind the last block are 0; open_block follows its block, or is -1.  The outputs may be
+ * the inputs themselves.  sink + recent <= keep, recent >= 1, num_blocks up to SBSA_CACHE8_MAX_BLOCKS. */
+int sbsa_cache8_evict(const int32_t* table, const float* weights, const int32_t* lengths,
+                      const int32_t* open_block, int32_t* table_out, float* weights_out,
+                      int32_t* lengths_out, int32_t* open_block_out, int num_seqs, int num_kv_heads,
+                      int num_blocks, int keep, int sink, int recent, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

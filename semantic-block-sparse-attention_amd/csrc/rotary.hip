@@ -1,0 +1,180 @@
+// Rotary positions of a layer's queries and keys, one launch for both.
+//
+// A pair (a, b) turns by t = position x frequency.  The angle is kept as a fraction of a
+// turn in 64-bit fixed point: position x turns mod 2^64 loses nothing at any position (in
+// fp32 the angle of position 10^6 would be off by 0.06), and the sine unit takes turns.
+//
+// A block takes one token (and a share of its heads): thread (unit, head) holds the sines
+// of its VEC pairs in registers and loops over heads, so they are made once for a
+// token and 1/HL of its heads.  A unit is VEC pairs (two vectors of VEC values), or VEC values that pass.
+#include "sbsa_common.h"
+
+namespace {
+
+struct RotaryArgs {
+  const bf16_t* q;
+  const bf16_t* k;
+  bf16_t* qo;
+  bf16_t* ko;
+  int64_t q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh;
+  const void* positions;
+  int64_t pos_axis, pos_stride;
+  const uint64_t* turns;
+  const uint8_t* axes;
+  float gain;
+  int pos_bytes, inverse;
+  int hq, hkv, rotary_dim, units, rot_units, unit_lanes, head_lanes;
+};
+
+template <int VEC>
+__device__ __forceinline__ void load_vec(const bf16_t* p, bf16_t (&x)[VEC]) {
+  if constexpr (VEC == 8) {
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(p);
+    __builtin_memcpy(x, &v, 16);
+  } else if constexpr (VEC == 2) {
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+    __builtin_memcpy(x, &v, 4);
+  } else {
+    x[0] = *p;
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_vec(bf16_t* p, const bf16_t (&x)[VEC]) {
+  if constexpr (VEC == 8) {
+    u32x4_t v;
+    __builtin_memcpy(&v, x, 16);
+    *reinterpret_cast<u32x4_t*>(p) = v;
+  } else if constexpr (VEC == 2) {
+    uint32_t v;
+    __builtin_memcpy(&v, x, 4);
+    *reinterpret_cast<uint32_t*>(p) = v;
+  } else {
+    *p = x[0];
+  }
+}
+
+template <int VEC, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+  const int64_t tok = blockIdx.x;
+  const int unit0 = threadIdx.x % a.unit_lanes;
+  const int hl = threadIdx.x / a.unit_lanes;
+  if (hl >= a.head_lanes) return;
+  const int heads = a.hq + a.hkv;
+  const int head_step = a.head_lanes * gridDim.y;
+  for (int u = unit0; u < a.units; u += a.unit_lanes) {
+    const bool rot = u < a.rot_units;
+    float c[VEC], s[VEC];
+    // the two vectors' places: (i, i + rotary_dim/2), neighbours, or one that passes
+    int d0, d1;
+    if (rot) {
+      d0 = INTERLEAVED ? 2 * VEC * u : VEC * u;
+      d1 = INTERLEAVED ? d0 + VEC : d0 + a.rotary_dim / 2;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int pair = VEC * u + i;
+        const int64_t at = (a.axes ? (int64_t)a.axes[pair] * a.pos_axis : 0) + tok * a.pos_stride;
+        const int64_t pos = a.pos_bytes == 8 ? reinterpret_cast<const int64_t*>(a.positions)[at]
+                                             : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[at];
+        const uint64_t angle = (uint64_t)pos * a.turns[pair];
+        const float t = (float)(int32_t)(angle >> 32) * 0x1p-32f;      // in [-1/2, 1/2] turns
+        c[i] = __builtin_amdgcn_cosf(t) * a.gain;
+        s[i] = __builtin_amdgcn_sinf(a.inverse ? -t : t) * a.gain;
+      }
+    } else {
+      d0 = d1 = a.rotary_dim + VEC * (u - a.rot_units);
+    }
+    for (int h = blockIdx.y * a.head_lanes + hl; h < heads; h += head_step) {
+      const bool is_q = h < a.hq;
+      const int hh = is_q ? h : h - a.hq;
+      const bf16_t* in = is_q ? a.q + tok * a.q_st + hh * a.q_sh : a.k + tok * a.k_st + hh * a.k_sh;
+      bf16_t* out = is_q ? a.qo + tok * a.qo_st + hh * a.qo_sh : a.ko + tok * a.ko_st + hh * a.ko_sh;
+      bf16_t x[VEC], y[VEC];
+      load_vec<VEC>(in + d0, x);
+      if (!rot) {
+        store_vec<VEC>(out + d0, x);
+        continue;
+      }
+      load_vec<VEC>(in + d1, y);
+      // x, y: first and second members where the pairs are apart, 2 VEC neighbours otherwise
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if constexpr (INTERLEAVED) {
+          bf16_t& pa = 2 * i < VEC ? x[2 * i] : y[2 * i - VEC];
+          bf16_t& pb = 2 * i + 1 < VEC ? x[2 * i + 1] : y[2 * i + 1 - VEC];
+          const float fa = bf2f(pa), fb = bf2f(pb);
+          pa = f2bf(fa * c[i] - fb * s[i]);
+          pb = f2bf(fb * c[i] + fa * s[i]);
+        } else {
+          const float fa = bf2f(x[i]), fb = bf2f(y[i]);
+          x[i] = f2bf(fa * c[i] - fb * s[i]);
+          y[i] = f2bf(fb * c[i] + fa * s[i]);
+        }
+      }
+      store_vec<VEC>(out + d0, x);
+      store_vec<VEC>(out + d1, y);
+    }
+  }
+}
+
+bool aligned(const void* p, int64_t st, int64_t sh, int vec) {
+  return ((uintptr_t)p % (2 * vec)) == 0 && st % vec == 0 && sh % vec == 0;
+}
+
+template <int VEC>
+void launch_rotary(RotaryArgs a, int64_t tokens, int head_dim, bool in_place, int interleaved, hipStream_t stream) {
+  a.rot_units = a.rotary_dim / (2 * VEC);
+  // what passes is there already where the outputs are the inputs
+  a.units = a.rot_units + (in_place ? 0 : (head_dim - a.rotary_dim) / VEC);
+  a.unit_lanes = a.units < 256 ? a.units : 256;
+  a.head_lanes = 256 / a.unit_lanes;
+  const int heads = a.hq + a.hkv;
+  if (a.head_lanes > heads) a.head_lanes = heads;
+  // few tokens: the heads over more blocks, until the blocks fill the card
+  int shares = (heads + a.head_lanes - 1) / a.head_lanes;
+  const int64_t most = 512 / tokens;
+  if (shares > most) shares = most < 1 ? 1 : (int)most;
+  const dim3 grid((unsigned)tokens, (unsigned)shares);
+  if (interleaved)
+    hipLaunchKernelGGL((rotary_kernel<VEC, true>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((rotary_kernel<VEC, false>), grid, dim3(256), 0, stream, a);
+}
+
+}  // namespace
+
+extern "C" int sbsa_rotary(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                           int num_q_heads, const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st,
+                           int64_t ko_sh, int num_kv_heads, const void* positions, int pos_bytes,
+                           int64_t pos_axis_stride, int64_t pos_stride, int64_t tokens, int head_dim, int rotary_dim,
+                           int interleaved, const uint64_t* turns, const uint8_t* axes, float gain, int inverse,
+                           hipStream_t stream) {
+  if (!q || !q_out || !positions || !turns || num_q_heads < 1 || num_kv_heads < 0 || tokens < 0 ||
+      (num_kv_heads > 0 && (!k || !k_out)) || (pos_bytes != 4 && pos_bytes != 8) || rotary_dim < 2 ||
+      rotary_dim % 2 || rotary_dim > head_dim || !(gain > 0.f))
+    return SBSA_ERR_ARG;
+  if (head_dim > 512 || tokens >= (1 << 24)) return SBSA_ERR_UNSUPPORTED;
+  if (tokens == 0) return SBSA_OK;
+  RotaryArgs a;
+  a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.qo = (bf16_t*)q_out; a.ko = (bf16_t*)k_out;
+  a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh;
+  a.qo_st = qo_st; a.qo_sh = qo_sh; a.ko_st = ko_st; a.ko_sh = ko_sh;
+  a.positions = positions; a.pos_axis = pos_axis_stride; a.pos_stride = pos_stride; a.pos_bytes = pos_bytes;
+  a.turns = turns; a.axes = axes; a.gain = inverse ? 1.f / gain : gain; a.inverse = inverse;
+  a.hq = num_q_heads; a.hkv = num_kv_heads; a.rotary_dim = rotary_dim;
+  const bool in_place = q == q_out && q_st == qo_st && q_sh == qo_sh &&
+                        (num_kv_heads == 0 || (k == k_out && k_st == ko_st && k_sh == ko_sh));
+  auto fits = [&](int vec) {
+    return rotary_dim % (2 * vec) == 0 && (head_dim - rotary_dim) % vec == 0 && aligned(q, q_st, q_sh, vec) &&
+           aligned(q_out, qo_st, qo_sh, vec) &&
+           (num_kv_heads == 0 || (aligned(k, k_st, k_sh, vec) && aligned(k_out, ko_st, ko_sh, vec)));
+  };
+  if (fits(8))
+    launch_rotary<8>(a, tokens, head_dim, in_place, interleaved, stream);
+  else if (fits(2))
+    launch_rotary<2>(a, tokens, head_dim, in_place, interleaved, stream);
+  else
+    launch_rotary<1>(a, tokens, head_dim, in_place, interleaved, stream);
+  SBSA_CHECK_LAUNCH();
+  return SBSA_OK;
+}

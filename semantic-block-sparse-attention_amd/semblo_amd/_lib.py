@@ -74,6 +74,12 @@ SIGNATURES = {
                                  P, I64, P]),
     "sbsa_gather_rows": (I32, [P, I64, I32, I32, P, I64, I64, I64, P, P, I64, I64, P]),
     "sbsa_repack_runs": (I32, [P, P, I64, I32, I32, I64, P, I64, P, P, I32, P, I64, P, I64, P]),
+    "sbsa_rotary": (I32, [P, I64, I64, P, I64, I64, I32, P, I64, I64, P, I64, I64, I32, P, I32, I64, I64, I64, I32,
+                          I32, I32, P, P, F32, I32, P]),
+    "sbsa_cache8_append": (I32, [P, P, I64, I64, P, I64, I64, I64, P, P, I64, P]),
+    "sbsa_cache8_attend_workspace_bytes": (SZ, [P, I32, I64, I64, I32, I32]),
+    "sbsa_cache8_attend": (I32, [P, P, I64, I64, I32, I64, P, I64, F32, P, I64, I64, P, I32, P, SZ, P]),
+    "sbsa_cache8_evict": (I32, [P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, I32, P]),
 }
 
 ERRORS = {1: "bad argument", 2: "unsupported shape", 3: "kernel launch failed",
@@ -132,3 +138,32 @@ def require_device(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("the semblo_amd kernels run on the GPU only (no CPU fallback)")
+
+
+def require_one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """Every tensor of a call lies on one ROCm device."""
+    require_device(first)
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise RuntimeError(f"one call's tensors lie on {device} and {t.device}")
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        if t.numel() == 0:
+            return 0, 0
+        first = t.data_ptr()
+        return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def call_on(device: torch.device, name: str, *args) -> int:
+    """``call`` with the device's current torch stream as the last argument, the device made current
+    for the launch where it is not."""
+    if device.type != "cuda" or device.index == torch.cuda.current_device():
+        return call(name, *args, stream(device))
+    with torch.cuda.device(device):
+        return call(name, *args, stream(device))

@@ -14,6 +14,7 @@
 #pragma once
 
 #include <stdint.h>
+#include <atomic>
 #include <cmath>
 #include <cstddef>
 #include <cstdio>
@@ -281,6 +282,43 @@ __forceinline__ void raw_buffer_store(T v, rsrc_t r, int voffset, int soffset) {
 }
 
 }  // namespace emu
+
+// ---- OCP e4m3 and the sine unit ----------------------------------------------
+namespace emu {
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16_pair;
+inline float e4m3_value(uint32_t c) {
+  const int e = (c >> 3) & 15, m = c & 7;
+  float v = e == 0 ? ldexpf((float)m, -9) : ldexpf(8.f + m, e - 10);
+  if (e == 15 && m == 7) v = NAN;
+  return c & 128 ? -v : v;
+}
+inline uint32_t e4m3_code(float f) {         // to nearest even; magnitudes past 448 give the NaN
+  const uint32_t sign = std::signbit(f) ? 128 : 0;
+  const float a = fabsf(f);
+  if (!(a < 464.f) && !(a == 464.f)) return sign | 127;
+  int e = a > 0.f ? ilogbf(a) : -6;
+  e = e < -6 ? -6 : e;
+  const float n = nearbyintf(ldexpf(a, 3 - e));      // 8 .. 16 (below 8: subnormal)
+  const uint32_t code = (uint32_t)((e + 6) * 8 + (int)n);
+  return sign | code;
+}
+inline bf16_pair cvt_pk_bf16_fp8(uint32_t w, float scale, bool hi) {
+  w >>= hi ? 16 : 0;
+  bf16_pair r;
+  r[0] = (__bf16)(e4m3_value(w & 255) * scale);
+  r[1] = (__bf16)(e4m3_value((w >> 8) & 255) * scale);
+  return r;
+}
+inline uint32_t cvt_pk_fp8_f32(float a, float b, uint32_t old, bool hi) {
+  const uint32_t v = e4m3_code(a) | (e4m3_code(b) << 8);
+  return hi ? (old & 0xffffu) | (v << 16) : (old & 0xffff0000u) | v;
+}
+}  // namespace emu
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, hi) emu::cvt_pk_bf16_fp8((w), (s), (hi))
+#define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, hi) emu::cvt_pk_fp8_f32((a), (b), (old), (hi))
+#define __builtin_amdgcn_sinf(x) ((float)sin(2 * M_PI * (double)(x)))
+#define __builtin_amdgcn_cosf(x) ((float)cos(2 * M_PI * (double)(x)))
+inline void __threadfence() { std::atomic_thread_fence(std::memory_order_seq_cst); }
 
 // ---- the builtins, mapped onto the emulation -----------------------------------
 #define __builtin_amdgcn_readfirstlane(x) emu::readfirstlane(x)
