@@ -499,7 +499,7 @@ int sbsa_cache8_append(const sbsa_cache8* cache, const void* k, int64_t k_st, in
 
 /* Attention of each sequence's newest tokens over its cache: row i of its n rows sees the first
  * length - n + i + 1 tokens; a row that sees none gives 0 and -inf.  q, out [tokens, Hq, dim] bf16,
- * lse [tokens, Hq] (natural; null only where accumulate is 0).  accumulate: weights[s, h, b] += the
+ * lse [tokens, Hq] (natural; or null).  accumulate: weights[s, h, b] += the
  * probabilities of block b's tokens over the rows and the head's query heads.  Rows of no sequence
  * keep what out and lse held.  Hq / Hkv up to 16, dim 128 or 256.  max_rows: a hint as in append. */
 size_t sbsa_cache8_attend_workspace_bytes(const sbsa_cache8* cache, int num_q_heads, int64_t tokens,

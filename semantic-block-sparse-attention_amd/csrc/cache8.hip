@@ -9,12 +9,25 @@
 namespace {
 
 constexpr int KB = SBSA_CACHE8_BLOCK;
+constexpr int BUFFER_CONFIG = 0x00020000;   // raw buffer resource, 32-bit data format
 constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float FLT_MOST = 3.402823466e38f;
 constexpr float LN2 = 0.69314718055994530942f;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
 
-__device__ __forceinline__ f32x16_t mfma32x32x16(bf16x8_t a, bf16x8_t b, f32x16_t c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f16x8_t as_f16x8(u32x4_t v) {
+  f16x8_t r;
+  __builtin_memcpy(&r, &v, 16);
+  return r;
+}
+
+__device__ __forceinline__ uint32_t pack2h(float a, float b) {
+  const f16x2_t v = __builtin_convertvector(f32x2_t{a, b}, f16x2_t);
+  uint32_t r;
+  __builtin_memcpy(&r, &v, 4);
+  return r;
 }
 
 // Four codes of a word as bf16 (exact: e4m3 has 4 significant bits, int8 7).
@@ -39,6 +52,38 @@ __device__ __forceinline__ bf16x8_t decode8(uint32_t w0, uint32_t w1) {
   decode4<FMT>(w1, c, d);
   r.x = a; r.y = b; r.z = c; r.w = d;
   return as_bf16x8(r);
+}
+
+// Four codes of a word as fp16 (exact too).
+template <int FMT>
+__device__ __forceinline__ void decode4h(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  f16x2_t a, b;
+  if constexpr (FMT == SBSA_CACHE8_E4M3) {
+    a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+    b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+  } else {
+    // code + 128 under the exponent of 1024 is the fp16 number 1152 + code
+    const uint32_t u = w ^ 0x80808080u;
+    const uint32_t x = __builtin_amdgcn_perm(0x64646464u, u, 0x07010700u);
+    const uint32_t y = __builtin_amdgcn_perm(0x64646464u, u, 0x07030702u);
+    const f16x2_t off = {(_Float16)1152.f, (_Float16)1152.f};
+    __builtin_memcpy(&a, &x, 4);
+    __builtin_memcpy(&b, &y, 4);
+    a -= off;
+    b -= off;
+  }
+  __builtin_memcpy(&lo, &a, 4);
+  __builtin_memcpy(&hi, &b, 4);
+}
+
+template <int FMT>
+__device__ __forceinline__ f16x8_t decode8h(uint32_t w0, uint32_t w1) {
+  u32x4_t r;
+  uint32_t a, b, c, d;
+  decode4h<FMT>(w0, a, b);
+  decode4h<FMT>(w1, c, d);
+  r.x = a; r.y = b; r.z = c; r.w = d;
+  return as_f16x8(r);
 }
 
 template <int FMT>
@@ -247,7 +292,10 @@ struct AttendArgs {
   int64_t o_st, o_sh;
   float* lse;                  // [tokens, Hq], natural
   float* part_o;               // [splits][tokens * Hq][D]
-  float* part_lse;             // [splits][tokens * Hq], base 2
+  // Sums of exponentials are kept as (m, l), 2^m l: the logarithm of one would round a weight by 10^-6
+  f32x2_t* part_ml;            // [splits][tokens * Hq]
+  f32x2_t* row_ml;             // [tokens * Hq], with 1 / l (accumulating)
+  f32x2_t* part_w;             // [tokens * Hq][N]: each block's sum of a row (few rows, accumulating)
   const int32_t* offsets;
   int64_t tokens, uniform;
   int hq, g, splits, tile_queries, tiles_per_seq;
@@ -273,13 +321,14 @@ __device__ __forceinline__ bool tile_of(const AttendArgs& a, int64_t t, int& s, 
     const int upto = wave_incl_scan(mine);
     const unsigned long long past = __ballot(before + upto > t);
     if (past) {
-      const int l = __ffsll((long long)past) - 1;
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)past) - 1);
       s = s0 + l;
       rows_of(a.offsets, s, 0, a.tokens, row0, n);
-      q0 = (int)(t - before - (__shfl(upto, l, 64) - __shfl(mine, l, 64))) * a.tile_queries;
+      const int upto_l = __builtin_amdgcn_readlane(upto, l), mine_l = __builtin_amdgcn_readlane(mine, l);
+      q0 = (int)(t - before - (upto_l - mine_l)) * a.tile_queries;
       return true;
     }
-    before += __shfl(upto, 63, 64);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
@@ -294,10 +343,20 @@ __device__ __forceinline__ u32x4_t clear_past(u32x4_t w, int keep) {
   return w;
 }
 
+__device__ __forceinline__ void finish_row(const AttendArgs& a, int64_t row, float m, float l) {
+  if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+  if (a.row_ml) a.row_ml[row] = f32x2_t{m, l == 0.f ? 0.f : 1.f / l};
+}
+
 // A wave's state over R = 16 or 32 rows (columns of S^T and O^T).  Lane l holds row l % R, and of
 // a block's 64 keys those of its part l / R: 16 or 32 consecutive ones, because the K rows
 // are handed to the product in the order that leaves them so.  They are the B operand of
 // O^T = V^T P^T as they lie, so the probabilities never leave the lane.
+//
+// P times the values' scale is rounded to fp16 (2^-11; bf16 would double the result's error).  For
+// fp16's range the scale is taken relative to the largest so far (v_ref) and times 2^11: with the reference
+// maximum at most 2^4 below the true one a probability is at most 2^15, and keeps its 11 bits down to 2^-25 of
+// the largest block's.
 template <int D, int FMT, int R>
 struct WaveRows {
   static constexpr int PARTS = 64 / R;          // lanes that share a row
@@ -306,35 +365,42 @@ struct WaveRows {
   static constexpr int SEG = 16 * PARTS;        // dims that one 16-byte load of every part covers
   static constexpr int NT = D / R;              // R-dim tiles of O^T
   static constexpr int NI = R * R / 64;         // accumulator values of a lane
+  static constexpr float P_SCALE = 0x1p11f, SLACK = 4.f;
   typedef __attribute__((ext_vector_type(NI))) float acc_t;
+  typedef u32x4_t kcodes_t[GROUPS][D / SEG];
+  typedef u32x4_t vcodes_t[NT][MINE / 16];
 
-  bf16x8_t q[D / SEG][2];
   acc_t o[NT];
   float m, l;
+  float v_ref;
 
   static __device__ __forceinline__ acc_t mfma(bf16x8_t x, bf16x8_t y, acc_t z) {
     if constexpr (R == 16)
-      return mfma16x16x32(x, y, z);
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, z, 0, 0, 0);
     else
-      return mfma32x32x16(x, y, z);
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, z, 0, 0, 0);
+  }
+  static __device__ __forceinline__ acc_t mfma(f16x8_t x, f16x8_t y, acc_t z) {
+    if constexpr (R == 16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, z, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, z, 0, 0, 0);
   }
 
-  __device__ __forceinline__ void start(const bf16_t* qrow, int lane) {
-    const int part = lane / R;
-#pragma unroll
-    for (int j = 0; j < D / SEG; ++j)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        u32x4_t w = {0u, 0u, 0u, 0u};
-        if (qrow) w = *reinterpret_cast<const u32x4_t*>(qrow + j * SEG + part * 16 + x * 8);
-        q[j][x] = as_bf16x8(w);
-      }
+  __device__ __forceinline__ void start() {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < NI; ++i) o[t][i] = 0.f;
     m = -INFINITY;
     l = 0.f;
+    v_ref = 0.f;
+  }
+
+  // piece x (of 2) of 16-byte step j of a row, for the lane's part; zeros without a row
+  static __device__ __forceinline__ u32x4_t query_piece(const bf16_t* qrow, int j, int x, int lane) {
+    const u32x4_t zero = {0u, 0u, 0u, 0u};
+    return qrow ? *reinterpret_cast<const u32x4_t*>(qrow + j * SEG + (lane / R) * 16 + x * 8) : zero;
   }
 
   // the key (of a block's 64) that row r of product g takes
@@ -345,35 +411,59 @@ struct WaveRows {
       return ((r >> 2) & 1) * 32 + g * 16 + (r >> 3) * 4 + (r & 3);
   }
 
-  // scores of a block's keys, times the keys' scale and log2(e) sm_scale
-  static __device__ __forceinline__ void scores(const bf16x8_t (&q)[D / SEG][2], const uint8_t* kb, float ks, int lane,
-                                                acc_t (&sc)[GROUPS]) {
-    const int part = lane / R;
+  // A block's codes through a buffer resource of its size: the address of a load is a scalar base, one lane
+  // offset and a scalar or literal one.  (By pointers the compiler carries 64-bit lane addresses and spills.)
+  static __device__ __forceinline__ void load_k(const uint8_t* kb, int lane, kcodes_t& kc) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)kb, 0, KB * D, BUFFER_CONFIG);
+    const int off = key_of(lane % R, 0) * D + (lane / R) * 16;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      const uint8_t* row = kb + key_of(lane % R, g) * D + part * 16;
-      acc_t acc;
+    for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-      for (int i = 0; i < NI; ++i) acc[i] = 0.f;
+      for (int j = 0; j < D / SEG; ++j)
+        kc[g][j] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + j * SEG, key_of(0, g) * D, 0);
+  }
+  static __device__ __forceinline__ void load_v(const uint8_t* vb, int lane, vcodes_t& vc) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)vb, 0, KB * D, BUFFER_CONFIG);
+    const int off = (lane % R) * KB + (lane / R) * MINE;
 #pragma unroll
-      for (int j = 0; j < D / SEG; ++j) {
-        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + j * SEG);
-        acc = mfma(decode8<FMT>(w.x, w.y), q[j][0], acc);
-        acc = mfma(decode8<FMT>(w.z, w.w), q[j][1], acc);
-      }
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < NI; ++i) acc[i] *= ks;
-      sc[g] = acc;
-    }
+      for (int x = 0; x < MINE / 16; ++x)
+        vc[t][x] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + x * 16, t * R * KB, 0);
   }
 
-  // one block: seen is how many of its keys the lane's row sees, filled how many are there (all: every row
-  // sees every key)
-  __device__ __forceinline__ void block(const uint8_t* kb, const uint8_t* vb, float ks, float vs, int seen, int filled,
-                                        bool all, int lane) {
+  // scores of a block's keys, times ks; q(j, x) gives the rows' pieces
+  template <class Q>
+  static __device__ __forceinline__ void scores(const kcodes_t& kc, Q&& q, float ks, acc_t (&sc)[GROUPS]) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) sc[g][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / SEG; ++j)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const bf16x8_t qq = as_bf16x8(q(j, x));
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          u32x4_t w = kc[g][j];
+          asm volatile("" : "+v"(w));           // decoded here, not where it was loaded
+          sc[g] = mfma(x ? decode8<FMT>(w.z, w.w) : decode8<FMT>(w.x, w.y), qq, sc[g]);
+        }
+        // without these the compiler decodes far ahead and runs out of registers
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) sc[g][i] *= ks;
+  }
+
+  // a block's scores to probabilities p (fp16, with the values' scale), the state moved on.  seen: how
+  // many of its keys the lane's row sees (all: every row every one).  Returns the lane's sum.
+  __device__ __forceinline__ float softmax(acc_t (&sc)[GROUPS], float vs, int seen, bool all, int lane,
+                                           u32x4_t (&p)[MINE / 8]) {
     const int part = lane / R;
-    acc_t sc[GROUPS];
-    scores(q, kb, ks, lane, sc);
     if (!all) {
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
@@ -388,213 +478,369 @@ struct WaveRows {
       for (int i = 0; i < NI; ++i) top = fmaxf(top, sc[g][i]);
     if constexpr (R == 16) top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    // the reference maximum moves only when a row has gone 2^8 above it: until then its
-    // probabilities are at most 2^8, which neither bf16 nor the fp32 sums mind
-    if (__ballot(top > m + 8.f)) {
+    // the reference maximum moves only when a row has gone 2^SLACK above it, the reference
+    // scale when a block's is larger
+    if (__ballot(top > m + SLACK || fabsf(vs) > v_ref)) {
+      // a score past fp32's range counts as its largest number (infinities would leave NaN)
+      if (__ballot(top == INFINITY)) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+          for (int i = 0; i < NI; ++i) sc[g][i] = sc[g][i] == INFINITY ? FLT_MOST : sc[g][i];
+        top = top == INFINITY ? FLT_MOST : top;
+      }
       const float to = fmaxf(m, top);
-      const float f = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to);
+      float f = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to);
       l *= f;
+      m = to;
+      if (fabsf(vs) > v_ref) {
+        f *= v_ref / fabsf(vs);
+        v_ref = fabsf(vs);
+      }
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < NI; ++i) o[t][i] *= f;
-      m = to;
     }
     const float ref = m == -INFINITY ? 0.f : m;
-    u32x4_t p[MINE / 8];
+    const float pv = v_ref > 0.f ? vs / v_ref * P_SCALE : vs * 0.f;       // a NaN scale stays one
+    float sum = 0.f;
 #pragma unroll
     for (int x = 0; x < MINE / 2; ++x) {
       const int i0 = 2 * x, i1 = 2 * x + 1;
       const float p0 = __builtin_amdgcn_exp2f(sc[i0 / NI][i0 % NI] - ref);
       const float p1 = __builtin_amdgcn_exp2f(sc[i1 / NI][i1 % NI] - ref);
-      l += p0 + p1;
-      // the scale joins the probability before its one rounding; an unseen key's is 0 whatever the scale
+      sum += p0 + p1;
+      // an unseen key's product is 0 whatever the scale
       const bool h0 = !all && part * MINE + i0 >= seen, h1 = !all && part * MINE + i1 >= seen;
-      p[x / 4][x % 4] = pack2bf(h0 ? 0.f : p0 * vs, h1 ? 0.f : p1 * vs);
+      p[x / 4][x % 4] = pack2h(h0 ? 0.f : p0 * pv, h1 ? 0.f : p1 * pv);
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const uint8_t* row = vb + (t * R + lane % R) * KB + part * MINE;
-#pragma unroll
-      for (int x = 0; x < MINE / 16; ++x) {
-        u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + x * 16);
-        if (!all) w = clear_past(w, filled - (part * MINE + x * 16));
-        o[t] = mfma(decode8<FMT>(w.x, w.y), as_bf16x8(p[2 * x]), o[t]);
-        o[t] = mfma(decode8<FMT>(w.z, w.w), as_bf16x8(p[2 * x + 1]), o[t]);
-      }
-    }
+    l += sum;
+    return sum;
   }
 
-  // the row's sum over its lanes
+  // filled: how many of the block's keys are there
+  __device__ __forceinline__ void values(vcodes_t& vc, const u32x4_t (&p)[MINE / 8], int filled, int lane) {
+    if (filled < KB) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int x = 0; x < MINE / 16; ++x) vc[t][x] = clear_past(vc[t][x], filled - ((lane / R) * MINE + x * 16));
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < MINE / 16; ++x) {
+        u32x4_t w = vc[t][x];
+        asm volatile("" : "+v"(w));
+        o[t] = mfma(decode8h<FMT>(w.x, w.y), as_f16x8(p[2 * x]), o[t]);
+        o[t] = mfma(decode8h<FMT>(w.z, w.w), as_f16x8(p[2 * x + 1]), o[t]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+
+  // the row's sum over its lanes, and O as the wave's own result (normalised before it gets the values'
+  // unit back, or a sum of large values would pass fp32's range).  A row without keys has sum 0 and gives 0; a NaN stays one.
   __device__ __forceinline__ void total() {
     if constexpr (R == 16) l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-  }
-
-  // joins another wave's rows, left in LDS
-  static constexpr int FOLD_FLOATS = NT * NI * 64 + 128;
-  __device__ __forceinline__ void leave(float* to, int lane) const {
+    const float f = l == 0.f ? 0.f : 1.f / P_SCALE / l;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < NI; ++i) to[(t * NI + i) * 64 + lane] = o[t][i];
-    to[NT * NI * 64 + lane] = m;
-    to[NT * NI * 64 + 64 + lane] = l;
-  }
-  __device__ __forceinline__ void join(const float* from, int lane) {
-    const float m1 = from[NT * NI * 64 + lane], l1 = from[NT * NI * 64 + 64 + lane];
-    const float to = fmaxf(m, m1), ref = to == -INFINITY ? 0.f : to;
-    const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(m1 - ref);
-    m = to;
-    l = l * f0 + l1 * f1;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < NI; ++i) o[t][i] = o[t][i] * f0 + from[(t * NI + i) * 64 + lane] * f1;
+      for (int i = 0; i < NI; ++i) o[t][i] = o[t][i] * f * v_ref;
   }
 
   // four consecutive dims of the lane's row: tile t, quarter x of the accumulator
   static __device__ __forceinline__ int dim_of(int t, int x, int lane) { return t * R + 8 * x + 4 * (lane / R); }
+
+  // where a row's result goes: out, or its share's partial row
+  static __device__ __forceinline__ void store(const AttendArgs& a, int split, int64_t token, int head, int t, int x,
+                                               int lane, f32x4_t v) {
+    if (a.splits == 1) {
+      u32x2_t w;
+      w.x = pack2bf(v.x, v.y);
+      w.y = pack2bf(v.z, v.w);
+      *reinterpret_cast<u32x2_t*>(a.out + token * a.o_st + head * a.o_sh + dim_of(t, x, lane)) = w;
+    } else {
+      const int64_t row = (split * a.tokens + token) * a.hq + head;
+      *reinterpret_cast<f32x4_t*>(a.part_o + row * D + dim_of(t, x, lane)) = v;
+    }
+  }
+  // m, l: a row without keys has l = 0
+  static __device__ __forceinline__ void store_sum(const AttendArgs& a, int split, int64_t token, int head, float m, float l) {
+    const int64_t row = token * a.hq + head;
+    if (a.splits > 1)
+      a.part_ml[split * a.tokens * a.hq + row] = f32x2_t{m, l};
+    else
+      finish_row(a, row, m, l);
+  }
 };
 
-// One grid block: a tile of rows of one (sequence, KV head) over one share of the keys.  KEYS: its
-// four waves hold the same R rows and take every fourth block of keys each, joined through LDS at
-// the end; otherwise each holds R rows of its own.
-template <int D, int FMT, int R, bool KEYS>
-__global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_kernel(AttendArgs a) {
+// This lane's row of a tile, what it sees, and the tile's share of the blocks.
+template <int R>
+struct LaneRow {
+  int qi, head, vis, vis_most, vis_least, lo, hi, held;
+  bool there;
+  int64_t sh;
+
+  __device__ __forceinline__ void find(const AttendArgs& a, int s, int h, int n, int q0, int r, int split) {
+    sh = (int64_t)s * a.c.num_kv_heads + h;
+    held = __builtin_amdgcn_readfirstlane(held_of(a.c, sh));
+    qi = q0 + r / a.g;
+    head = h * a.g + r % a.g;
+    there = r < a.tile_queries * a.g && qi < n;
+    vis = there ? held - n + qi + 1 : 0;
+    vis = vis < 0 ? 0 : vis;
+    vis_most = vis;
+    vis_least = there ? vis : 0x7fffffff;
+#pragma unroll
+    for (int x = 1; x < R; x <<= 1) {
+      vis_most = max(vis_most, __shfl_xor(vis_most, x, 64));
+      vis_least = min(vis_least, __shfl_xor(vis_least, x, 64));
+    }
+    vis_most = __builtin_amdgcn_readfirstlane(vis_most);
+    vis_least = __builtin_amdgcn_readfirstlane(vis_least);
+    // the share: of the blocks that the tile's last row sees
+    const int tile_last = q0 + a.tile_queries < n ? q0 + a.tile_queries : n;
+    const int tile_vis = held - n + tile_last;
+    const int blocks = tile_vis > 0 ? (tile_vis + KB - 1) / KB : 0;
+    const int per = (blocks + a.splits - 1) / a.splits;
+    lo = split * per;
+    hi = lo + per < blocks ? lo + per : blocks;
+  }
+};
+
+// Few rows per sequence: a tile of R rows over one share of the keys, every fourth block of keys to each
+// wave, the waves joined through LDS.  The codes go from memory to the registers that the products read,
+// the next block's on their way while this one's are used; no barrier and no LDS traffic but the queries'.
+template <int D, int FMT, int R>
+__global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_keys_kernel(AttendArgs a) {
   using W = WaveRows<D, FMT, R>;
+  constexpr int TILE = W::NT * W::NI * 64;          // floats of a wave's O
+  constexpr int PIECES = D / W::SEG * 2;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem_keys[];
+  float* fold = reinterpret_cast<float*>(smem_keys);
+  __shared__ u32x4_t sq[PIECES * 64];
+  __shared__ float sm[4 * 64], sl[4 * 64];
   const sbsa_cache8& c = a.c;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int split = (int)(blockIdx.x % a.splits);
   const int64_t tiles = gridDim.x / a.splits;
-  __shared__ float fold[KEYS ? W::FOLD_FLOATS : 1];
+  int s, n, q0;
+  int64_t row0;
+  if (!tile_of(a, tiles - 1 - blockIdx.x / a.splits, s, row0, n, q0)) return;
+  LaneRow<R> r;
+  r.find(a, s, (int)blockIdx.y, n, q0, lane % R, split);
+  const int64_t token = row0 + r.qi;
+  const bf16_t* qrow = r.there ? a.q + token * a.q_st + r.head * a.q_sh : nullptr;
+  for (int i = wave; i < PIECES; i += 4) sq[i * 64 + lane] = W::query_piece(qrow, i >> 1, i & 1, lane);
 
+  W w;
+  w.start();
+  const int64_t heads = (int64_t)c.num_seqs * c.num_kv_heads;
+  const int64_t base = r.sh * c.num_blocks;
+  const uint8_t* codes_k = (const uint8_t*)c.codes_k + base * KB * D;
+  const uint8_t* codes_v = (const uint8_t*)c.codes_v + base * KB * D;
+  const int first = r.lo + wave;
+  const int count = r.hi > first ? (r.hi - first + 3) / 4 : 0;
+  // the places and scales of the wave's next 64 blocks, one per lane
+  int place = 0;
+  float ks = 0.f, vs = 0.f;
+  auto fetch = [&](int i0) {
+    const int b = first + 4 * (i0 + lane);
+    place = 0;
+    if (b < r.hi) {
+      place = (int)(place_of(c, r.sh, b) - base);
+      ks = c.scales[base + place] * a.scale_log2;
+      vs = c.scales[heads * c.num_blocks + base + place];
+    }
+  };
+  typename W::kcodes_t kc;
+  typename W::vcodes_t vc;
+  if (count > 0) {
+    fetch(0);
+    const int64_t at = (int64_t)__builtin_amdgcn_readlane(place, 0) * (KB * D);
+    W::load_k(codes_k + at, lane, kc);
+    W::load_v(codes_v + at, lane, vc);
+  }
+  __syncthreads();                                  // the queries are in LDS
+  for (int i = 0; i < count; ++i) {
+    const int b = first + 4 * i;
+    const float ksi = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(ks), i & 63));
+    const float vsi = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(vs), i & 63));
+    if (((i + 1) & 63) == 0) fetch(i + 1);
+    const int64_t at = (int64_t)__builtin_amdgcn_readlane(place, (i + 1) & 63) * (KB * D);
+    typename W::acc_t sc[W::GROUPS];
+    W::scores(kc, [&](int j, int x) { return sq[(2 * j + x) * 64 + lane]; }, ksi, sc);
+    if (i + 1 < count) W::load_k(codes_k + at, lane, kc);
+    u32x4_t p[W::MINE / 8];
+    float sum = w.softmax(sc, vsi, r.vis - b * KB, (b + 1) * KB <= r.vis_least, lane, p);
+    if (a.part_w) {
+      // the block's share of each row's attention, for the blocks' weights
+      if constexpr (R == 16) sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if (r.there && lane < R)
+        a.part_w[(token * a.hq + r.head) * c.num_blocks + b] = f32x2_t{w.m, sum};
+    }
+    w.values(vc, p, r.held - b * KB, lane);
+    if (i + 1 < count) W::load_v(codes_v + at, lane, vc);
+    asm volatile("" ::: "memory");                  // the queries stay in LDS, not in registers
+  }
+  w.total();
+#pragma unroll
+  for (int t = 0; t < W::NT; ++t)
+#pragma unroll
+    for (int i = 0; i < W::NI; ++i) fold[wave * TILE + (t * W::NI + i) * 64 + lane] = w.o[t][i];
+  sm[wave * 64 + lane] = w.m;
+  sl[wave * 64 + lane] = w.l;
+  __syncthreads();
+  // each wave joins a quarter of the dims
+  float top = -INFINITY, f[4], total = 0.f;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) top = fmaxf(top, sm[x * 64 + lane]);
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    f[x] = sl[x * 64 + lane] * __builtin_amdgcn_exp2f(sm[x * 64 + lane] - ref);
+    total += f[x];
+  }
+  if (!r.there) return;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) f[x] *= inv;
+  constexpr int OWN = W::NT / 4;
+#pragma unroll
+  for (int tt = 0; tt < OWN; ++tt) {
+    const int t = wave * OWN + tt;
+#pragma unroll
+    for (int q = 0; q < W::NI / 4; ++q) {
+      f32x4_t v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = (t * W::NI + 4 * q + i) * 64 + lane;
+        v[i] = (fold[at] * f[0] + fold[TILE + at] * f[1]) + (fold[2 * TILE + at] * f[2] + fold[3 * TILE + at] * f[3]);
+      }
+      W::store(a, split, token, r.head, t, q, lane, v);
+    }
+  }
+  if (wave == 0 && lane < R) W::store_sum(a, split, token, r.head, top, total);
+}
+
+// Many rows: 32 of them to each wave, over one share of the keys.
+template <int D, int FMT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_rows_kernel(AttendArgs a) {
+  using W = WaveRows<D, FMT, 32>;
+  const sbsa_cache8& c = a.c;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int split = (int)(blockIdx.x % a.splits);
+  const int64_t tiles = gridDim.x / a.splits;
   int s, n, q0;
   int64_t row0;
   // late tiles see the most keys: they go first
   if (!tile_of(a, tiles - 1 - blockIdx.x / a.splits, s, row0, n, q0)) return;
-  const int h = blockIdx.y;
-  const int64_t sh = (int64_t)s * c.num_kv_heads + h;
-  const int64_t heads = (int64_t)c.num_seqs * c.num_kv_heads;
-  const int held = held_of(c, sh);
-
-  // this lane's row
-  const int r = (KEYS ? 0 : wave * R) + lane % R;
-  const int qi = q0 + r / a.g, head = h * a.g + r % a.g;
-  const bool there = r < a.tile_queries * a.g && qi < n;
-  int vis = there ? held - n + qi + 1 : 0;
-  vis = vis < 0 ? 0 : vis;
-  int vis_most = vis, vis_least = there ? vis : 0x7fffffff;
+  LaneRow<32> r;
+  r.find(a, s, (int)blockIdx.y, n, q0, wave * 32 + lane % 32, split);
+  const int64_t token = row0 + r.qi;
+  const bf16_t* qrow = r.there ? a.q + token * a.q_st + r.head * a.q_sh : nullptr;
+  u32x4_t q[D / W::SEG][2];
 #pragma unroll
-  for (int x = 1; x < R; x <<= 1) {
-    vis_most = max(vis_most, __shfl_xor(vis_most, x, 64));
-    vis_least = min(vis_least, __shfl_xor(vis_least, x, 64));
-  }
-  vis_most = __builtin_amdgcn_readfirstlane(vis_most);
-  vis_least = __builtin_amdgcn_readfirstlane(vis_least);
-
-  // the share: of the blocks that the tile's last row sees
-  const int tile_last = q0 + a.tile_queries < n ? q0 + a.tile_queries : n;
-  int tile_vis = held - n + tile_last;
-  tile_vis = tile_vis < 0 ? 0 : tile_vis;
-  const int blocks = (tile_vis + KB - 1) / KB;
-  const int per = (blocks + a.splits - 1) / a.splits;
-  const int lo = split * per;
-  int hi = lo + per < blocks ? lo + per : blocks;
-  if (!KEYS) hi = min(hi, (vis_most + KB - 1) / KB);
-
+  for (int j = 0; j < D / W::SEG; ++j)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) q[j][x] = W::query_piece(qrow, j, x, lane);
   W w;
-  w.start(there ? a.q + (row0 + qi) * a.q_st + head * a.q_sh : nullptr, lane);
-  const float* scales_v = c.scales + heads * c.num_blocks;
-  for (int b = lo + (KEYS ? wave : 0); b < hi; b += KEYS ? 4 : 1) {
-    const int64_t place = place_of(c, sh, b);
-    w.block((const uint8_t*)c.codes_k + place * KB * D, (const uint8_t*)c.codes_v + place * KB * D,
-            c.scales[place] * a.scale_log2, scales_v[place], vis - b * KB, held - b * KB, (b + 1) * KB <= vis_least, lane);
+  w.start();
+  const int64_t heads = (int64_t)c.num_seqs * c.num_kv_heads;
+  const int hi = min(r.hi, (r.vis_most + KB - 1) / KB);
+  for (int b = r.lo; b < hi; ++b) {
+    const int64_t place = place_of(c, r.sh, b);
+    typename W::kcodes_t kc;
+    typename W::vcodes_t vc;
+    W::load_k((const uint8_t*)c.codes_k + place * (KB * D), lane, kc);
+    W::load_v((const uint8_t*)c.codes_v + place * (KB * D), lane, vc);
+    typename W::acc_t sc[W::GROUPS];
+    W::scores(kc, [&](int j, int x) { return q[j][x]; }, c.scales[place] * a.scale_log2, sc);
+    u32x4_t p[W::MINE / 8];
+    w.softmax(sc, c.scales[heads * c.num_blocks + place], r.vis - b * KB, (b + 1) * KB <= r.vis_least, lane, p);
+    w.values(vc, p, r.held - b * KB, lane);
   }
   w.total();
-  if constexpr (KEYS) {
-    for (int x = 3; x > 0; --x) {
-      if (wave == x) w.leave(fold, lane);
-      __syncthreads();
-      if (wave == 0) w.join(fold, lane);
-      __syncthreads();
-    }
-    if (wave != 0) return;
-  }
-  if (!there) return;
-  // a row without keys has sum 0 and gives 0; a NaN stays one
-  const float inv = w.l == 0.f ? 0.f : 1.f / w.l;
-  const float lse2 = w.l == 0.f ? -INFINITY : w.m + __builtin_amdgcn_logf(w.l);
-  const int64_t row = (row0 + qi) * a.hq + head;
-  if (a.splits == 1) {
-    bf16_t* out = a.out + (row0 + qi) * a.o_st + head * a.o_sh;
-#pragma unroll
-    for (int t = 0; t < W::NT; ++t)
-#pragma unroll
-      for (int x = 0; x < W::NI / 4; ++x) {
-        u32x2_t v;
-        v.x = pack2bf(w.o[t][4 * x] * inv, w.o[t][4 * x + 1] * inv);
-        v.y = pack2bf(w.o[t][4 * x + 2] * inv, w.o[t][4 * x + 3] * inv);
-        *reinterpret_cast<u32x2_t*>(out + W::dim_of(t, x, lane)) = v;
-      }
-    if (a.lse && lane < R) a.lse[row] = lse2 * LN2;
-    return;
-  }
-  float* po = a.part_o + ((int64_t)split * a.tokens * a.hq + row) * D;
+  if (!r.there) return;
 #pragma unroll
   for (int t = 0; t < W::NT; ++t)
 #pragma unroll
     for (int x = 0; x < W::NI / 4; ++x) {
       f32x4_t v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = w.o[t][4 * x + i] * inv;
-      *reinterpret_cast<f32x4_t*>(po + W::dim_of(t, x, lane)) = v;
+      for (int i = 0; i < 4; ++i) v[i] = w.o[t][4 * x + i];
+      W::store(a, split, token, r.head, t, x, lane, v);
     }
-  if (lane < R) a.part_lse[(int64_t)split * a.tokens * a.hq + row] = lse2;
+  if (lane < 32) W::store_sum(a, split, token, r.head, w.m, w.l);
 }
 
-// The shares of a row joined: a grid block per row, its waves every fourth share each.
+// The shares of a row joined: a grid block takes 64 dims of a row, 16 threads to a share's 64 dims and every
+// 16th share to each.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
-  constexpr int PER = D / 64;
   const int64_t row = blockIdx.x, rows = a.tokens * a.hq;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
   const int64_t token = row / a.hq;
   const int head = (int)(row % a.hq);
   if (a.offsets && (token < a.offsets[0] || token >= a.offsets[a.c.num_seqs])) return;
-  __shared__ float fold[4][64 * PER];
+  __shared__ f32x4_t fold[16 * 16];
+  const f32x2_t* ml = a.part_ml + row;
   float top = -INFINITY;
-  for (int x = lane; x < a.splits; x += 64) top = fmaxf(top, a.part_lse[x * rows + row]);
+  for (int x = lane; x < a.splits; x += 64) top = fmaxf(top, ml[x * rows].x);
   top = wave_max(top);
   const float ref = top == -INFINITY ? 0.f : top;
-  float total = 0.f, acc[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-  for (int x = lane; x < a.splits; x += 64) total += __builtin_amdgcn_exp2f(a.part_lse[x * rows + row] - ref);
+  float total = 0.f;
+  for (int x = lane; x < a.splits; x += 64) {
+    const f32x2_t v = ml[x * rows];
+    total += v.y * __builtin_amdgcn_exp2f(v.x - ref);
+  }
   total = wave_sum(total);
-  for (int x = wave; x < a.splits; x += 4) {
-    const float v = a.part_lse[x * rows + row];
-    if (v == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(v - ref);
-    const float* po = a.part_o + (x * rows + row) * D + lane * PER;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] += f * po[i];
-  }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) fold[wave][lane * PER + i] = acc[i];
-  __syncthreads();
-  if (wave != 0) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  bf16_t* out = a.out + token * a.o_st + head * a.o_sh + lane * PER;
-#pragma unroll
-  for (int i = 0; i < PER; i += 2) {
-    const int d = lane * PER + i;
-    const float x = (fold[0][d] + fold[1][d]) + (fold[2][d] + fold[3][d]);
-    const float y = (fold[0][d + 1] + fold[1][d + 1]) + (fold[2][d + 1] + fold[3][d + 1]);
-    *reinterpret_cast<uint32_t*>(out + i) = pack2bf(x * inv, y * inv);
+  const int d = (int)blockIdx.y * 64 + (threadIdx.x & 15) * 4;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int x = threadIdx.x >> 4; x < a.splits; x += 16) {
+    const f32x2_t v = ml[x * rows];
+    const f32x4_t o = *reinterpret_cast<const f32x4_t*>(a.part_o + (x * rows + row) * D + d);
+    acc += o * (v.y * __builtin_amdgcn_exp2f(v.x - ref) * inv);      // a share without keys has an O of 0
   }
-  if (a.lse && lane == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * LN2;
+  fold[threadIdx.x] = acc;
+  __syncthreads();
+  if (threadIdx.x >= 16) return;
+  f32x4_t sum = fold[threadIdx.x];
+  for (int x = 1; x < 16; ++x) sum += fold[x * 16 + threadIdx.x];
+  u32x2_t w;
+  w.x = pack2bf(sum.x, sum.y);
+  w.y = pack2bf(sum.z, sum.w);
+  *reinterpret_cast<u32x2_t*>(a.out + token * a.o_st + head * a.o_sh + d) = w;
+  if (threadIdx.x == 0 && blockIdx.y == 0) finish_row(a, row, top, total);
+}
+
+// The blocks' weights from the shares that few rows left block by block: a thread per block.
+__global__ __launch_bounds__(256) void weigh_shares_kernel(AttendArgs a) {
+  const sbsa_cache8& c = a.c;
+  const int b = (int)(blockIdx.x * 256 + threadIdx.x), h = blockIdx.y, s = blockIdx.z;
+  const int64_t sh = (int64_t)s * c.num_kv_heads + h;
+  int64_t row0;
+  int n;
+  rows_of(a.offsets, s, a.uniform, a.tokens, row0, n);
+  const int held = held_of(c, sh);
+  if (n == 0 || b * KB >= held) return;
+  float sum = 0.f;
+  int qi = b * KB - (held - n);                      // the first row that sees the block
+  for (qi = qi < 0 ? 0 : qi; qi < n; ++qi)
+    for (int j = 0; j < a.g; ++j) {
+      const int64_t row = (row0 + qi) * a.hq + h * a.g + j;
+      const f32x2_t w = a.part_w[row * c.num_blocks + b], all = a.row_ml[row];
+      sum += w.y == 0.f ? 0.f : w.y * __builtin_amdgcn_exp2f(w.x - all.x) * all.y;
+    }
+  c.weights[sh * c.num_blocks + b] += sum;
 }
 
 // The attention that each block receives: a wave holds a block of keys and goes over the rows that
@@ -604,7 +850,7 @@ __global__ __launch_bounds__(256) void weigh_kernel(AttendArgs a) {
   using W = WaveRows<D, FMT, 32>;
   const sbsa_cache8& c = a.c;
   const int lane = threadIdx.x & 63;
-  const int b = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
+  const int b = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int h = blockIdx.y, s = blockIdx.z;
   const int64_t sh = (int64_t)s * c.num_kv_heads + h;
   int64_t row0;
@@ -613,7 +859,8 @@ __global__ __launch_bounds__(256) void weigh_kernel(AttendArgs a) {
   const int held = held_of(c, sh);
   if (n == 0 || b * KB >= held) return;
   const int64_t place = place_of(c, sh, b);
-  const uint8_t* kb = (const uint8_t*)c.codes_k + place * KB * D;
+  typename W::kcodes_t kc;
+  W::load_k((const uint8_t*)c.codes_k + place * (KB * D), lane, kc);
   const float ks = c.scales[place] * a.scale_log2;
   // the first row that sees the block's first key
   int first = b * KB - (held - n);
@@ -625,16 +872,16 @@ __global__ __launch_bounds__(256) void weigh_kernel(AttendArgs a) {
     const int64_t qi = there ? r / a.g : 0;
     const int head = h * a.g + (int)(r % a.g);
     const int seen = there ? (int)(held - n + qi + 1 - b * KB) : 0;
-    W w;
-    w.start(there ? a.q + (row0 + qi) * a.q_st + head * a.q_sh : nullptr, lane);
-    const float lse2 = there ? a.lse[(row0 + qi) * a.hq + head] * LOG2E : 0.f;
+    const bf16_t* qrow = there ? a.q + (row0 + qi) * a.q_st + head * a.q_sh : nullptr;
+    const f32x2_t none = {0.f, 0.f};
+    const f32x2_t all = there ? a.row_ml[(row0 + qi) * a.hq + head] : none;
     typename W::acc_t sc[W::GROUPS];
-    W::scores(w.q, kb, ks, lane, sc);
+    W::scores(kc, [&](int j, int x) { return W::query_piece(qrow, j, x, lane); }, ks, sc);
 #pragma unroll
     for (int g = 0; g < W::GROUPS; ++g)
 #pragma unroll
       for (int i = 0; i < W::NI; ++i)
-        sum += (lane / 32) * W::MINE + g * W::NI + i < seen ? __builtin_amdgcn_exp2f(sc[g][i] - lse2) : 0.f;
+        sum += (lane / 32) * W::MINE + g * W::NI + i < seen ? __builtin_amdgcn_exp2f(fminf(sc[g][i], FLT_MOST) - all.x) * all.y : 0.f;
   }
   sum = wave_sum(sum);
   if (lane == 0) c.weights[sh * c.num_blocks + b] += sum;
@@ -803,25 +1050,50 @@ AttendPlan plan_attend(const sbsa_cache8* c, int num_q_heads, int64_t tokens, in
   return p;
 }
 
-size_t attend_bytes(const AttendPlan& p, int64_t tokens, int num_q_heads, int dim) {
-  return p.splits > 1 ? (size_t)p.splits * tokens * num_q_heads * (dim + 1) * sizeof(float) : 0;
+// The workspace's parts, in floats: the shares' O and sums, the rows' sums, and each row's sums block by block.
+struct AttendSpace {
+  size_t o, part, row, w;
+  size_t bytes() const { return (o + part + row + w) * sizeof(float); }
+};
+
+AttendSpace attend_space(const AttendPlan& p, const sbsa_cache8* c, int64_t tokens, int num_q_heads, bool accumulate) {
+  const size_t rows = (size_t)tokens * num_q_heads;
+  AttendSpace x;
+  x.o = p.splits > 1 ? p.splits * rows * c->head_dim : 0;
+  x.part = p.splits > 1 ? 2 * p.splits * rows : 0;
+  x.row = accumulate ? 2 * rows : 0;
+  x.w = accumulate && p.keys ? 2 * rows * c->num_blocks : 0;
+  return x;
+}
+
+template <int D, int FMT, int R>
+bool launch_keys(const AttendArgs& a, dim3 grid, hipStream_t stream) {
+  constexpr int lds = 4 * R * D * (int)sizeof(float);
+  if (lds > 48 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(attend_keys_kernel<D, FMT, R>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    return false;
+  hipLaunchKernelGGL((attend_keys_kernel<D, FMT, R>), grid, dim3(256), lds, stream, a);
+  return true;
 }
 
 template <int D, int FMT>
-void launch_attend(const AttendArgs& a, const AttendPlan& p, int accumulate, hipStream_t stream) {
+bool launch_attend(const AttendArgs& a, const AttendPlan& p, int accumulate, hipStream_t stream) {
   const dim3 grid((unsigned)(p.tiles * p.splits), (unsigned)a.c.num_kv_heads);
-  if (p.keys && p.rows == 16)
-    hipLaunchKernelGGL((attend_kernel<D, FMT, 16, true>), grid, dim3(256), 0, stream, a);
-  else if (p.keys)
-    hipLaunchKernelGGL((attend_kernel<D, FMT, 32, true>), grid, dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((attend_kernel<D, FMT, 32, false>), grid, dim3(256), 0, stream, a);
+  if (p.keys) {
+    if (!(p.rows == 16 ? launch_keys<D, FMT, 16>(a, grid, stream) : launch_keys<D, FMT, 32>(a, grid, stream))) return false;
+  } else {
+    hipLaunchKernelGGL((attend_rows_kernel<D, FMT>), grid, dim3(256), 0, stream, a);
+  }
   if (p.splits > 1)
-    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.tokens * a.hq)), dim3(256), 0, stream, a);
-  if (accumulate)
+    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.tokens * a.hq), D / 64), dim3(256), 0, stream, a);
+  if (accumulate && p.keys)
+    hipLaunchKernelGGL(weigh_shares_kernel, dim3((unsigned)((a.c.num_blocks + 255) / 256), (unsigned)a.c.num_kv_heads,
+                                                 (unsigned)a.c.num_seqs), dim3(256), 0, stream, a);
+  else if (accumulate)
     hipLaunchKernelGGL((weigh_kernel<D, FMT>),
                        dim3((unsigned)((a.c.num_blocks + 3) / 4), (unsigned)a.c.num_kv_heads, (unsigned)a.c.num_seqs),
                        dim3(256), 0, stream, a);
+  return true;
 }
 
 }  // namespace
@@ -855,12 +1127,11 @@ extern "C" int sbsa_cache8_append(const sbsa_cache8* cache, const void* k, int64
 
 extern "C" size_t sbsa_cache8_attend_workspace_bytes(const sbsa_cache8* cache, int num_q_heads, int64_t tokens,
                                                      int64_t max_rows, int ragged, int accumulate) {
-  (void)accumulate;
   if (!cache || cache->num_seqs < 1 || cache->num_kv_heads < 1 || num_q_heads < cache->num_kv_heads ||
       num_q_heads / cache->num_kv_heads > 16 || tokens < 1)
     return 0;
-  return attend_bytes(plan_attend(cache, num_q_heads, tokens, max_rows, ragged != 0), tokens, num_q_heads,
-                      cache->head_dim);
+  return attend_space(plan_attend(cache, num_q_heads, tokens, max_rows, ragged != 0), cache, tokens, num_q_heads,
+                      accumulate != 0).bytes();
 }
 
 extern "C" int sbsa_cache8_attend(const sbsa_cache8* cache, const void* q, int64_t q_st, int64_t q_sh, int num_q_heads,
@@ -868,7 +1139,7 @@ extern "C" int sbsa_cache8_attend(const sbsa_cache8* cache, const void* q, int64
                                   int64_t o_st, int64_t o_sh, float* lse, int accumulate, void* workspace,
                                   size_t workspace_bytes, hipStream_t stream) {
   if (bad_cache(cache) || tokens < 0 || num_q_heads < 1 || num_q_heads % cache->num_kv_heads ||
-      (!offsets && tokens % cache->num_seqs) || (accumulate && !lse))
+      (!offsets && tokens % cache->num_seqs))
     return SBSA_ERR_ARG;
   if (tokens > 0 && (bad_rows(q, q_st, q_sh) || bad_rows(out, o_st, o_sh))) return SBSA_ERR_ARG;
   if (unsupported_cache(cache) || num_q_heads / cache->num_kv_heads > 16 || tokens * num_q_heads >= (1 << 24))
@@ -876,24 +1147,28 @@ extern "C" int sbsa_cache8_attend(const sbsa_cache8* cache, const void* q, int64
   if (tokens == 0) return SBSA_OK;
   const AttendPlan p = plan_attend(cache, num_q_heads, tokens, max_rows, offsets != nullptr);
   if (p.tiles * p.splits >= (1 << 24)) return SBSA_ERR_UNSUPPORTED;
-  if (workspace_bytes < attend_bytes(p, tokens, num_q_heads, cache->head_dim)) return SBSA_ERR_CAPACITY;
-  if (p.splits > 1 && (!workspace || (uintptr_t)workspace % 16)) return SBSA_ERR_ARG;
+  const AttendSpace space = attend_space(p, cache, tokens, num_q_heads, accumulate != 0);
+  if (workspace_bytes < space.bytes()) return SBSA_ERR_CAPACITY;
+  if (space.bytes() > 0 && (!workspace || (uintptr_t)workspace % 16)) return SBSA_ERR_ARG;
   AttendArgs a;
   a.c = *cache;
   a.q = (const bf16_t*)q; a.q_st = q_st; a.q_sh = q_sh;
   a.out = (bf16_t*)out; a.o_st = o_st; a.o_sh = o_sh; a.lse = lse;
   a.part_o = (float*)workspace;
-  a.part_lse = a.part_o + (size_t)p.splits * tokens * num_q_heads * cache->head_dim;
+  a.part_ml = (f32x2_t*)(a.part_o + space.o);
+  a.row_ml = accumulate ? (f32x2_t*)(a.part_o + space.o + space.part) : nullptr;
+  a.part_w = space.w ? (f32x2_t*)(a.part_o + space.o + space.part + space.row) : nullptr;
   a.offsets = offsets; a.tokens = tokens; a.uniform = tokens / cache->num_seqs;
   a.hq = num_q_heads; a.g = num_q_heads / cache->num_kv_heads;
   a.splits = p.splits; a.tile_queries = p.tile_queries; a.tiles_per_seq = p.tiles_per_seq;
   a.scale_log2 = sm_scale * LOG2E;
-  if (cache->head_dim == 128)
-    cache->format == SBSA_CACHE8_E4M3 ? launch_attend<128, SBSA_CACHE8_E4M3>(a, p, accumulate, stream)
-                                      : launch_attend<128, SBSA_CACHE8_INT8>(a, p, accumulate, stream);
-  else
-    cache->format == SBSA_CACHE8_E4M3 ? launch_attend<256, SBSA_CACHE8_E4M3>(a, p, accumulate, stream)
-                                      : launch_attend<256, SBSA_CACHE8_INT8>(a, p, accumulate, stream);
+  const bool e4m3 = cache->format == SBSA_CACHE8_E4M3;
+  const bool ok = cache->head_dim == 128
+                      ? (e4m3 ? launch_attend<128, SBSA_CACHE8_E4M3>(a, p, accumulate, stream)
+                              : launch_attend<128, SBSA_CACHE8_INT8>(a, p, accumulate, stream))
+                      : (e4m3 ? launch_attend<256, SBSA_CACHE8_E4M3>(a, p, accumulate, stream)
+                              : launch_attend<256, SBSA_CACHE8_INT8>(a, p, accumulate, stream));
+  if (!ok) return SBSA_ERR_LAUNCH;
   SBSA_CHECK_LAUNCH();
   return SBSA_OK;
 }

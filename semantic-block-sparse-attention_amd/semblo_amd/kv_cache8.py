@@ -249,7 +249,7 @@ class QuantizedKVCache:
             raise ValueError(f"out must be bfloat16 {list(q.shape)} with rows on 16 bytes")
         elif _lib.overlap(out, q):
             raise ValueError("out overlaps q")
-        lse = torch.empty((tokens, hq), dtype=torch.float32, device=q.device) if return_lse or accumulate else None
+        lse = torch.empty((tokens, hq), dtype=torch.float32, device=q.device) if return_lse else None
         _lib.require_one_device(self.codes_k, q, out, offsets)
         need = _lib.query("sbsa_cache8_attend_workspace_bytes", self._ref, hq, tokens, hint, int(at is not None),
                           int(accumulate))

@@ -280,6 +280,15 @@ template <class T>
 __forceinline__ void raw_buffer_store(T v, rsrc_t r, int voffset, int soffset) {
   buffer_store(r.w, voffset + soffset, &v, sizeof(T));
 }
+typedef __attribute__((ext_vector_type(4))) uint32_t emu_u32x4_t;
+// bytes past the resource's range read as 0
+inline emu_u32x4_t raw_buffer_load_b128(rsrc_t r, int voffset, int soffset) {
+  const uint64_t base = r.w[0] | ((uint64_t)(r.w[1] & 0xffffu) << 32);
+  const uint64_t off = (uint64_t)(uint32_t)voffset + (uint32_t)soffset;
+  emu_u32x4_t v = {0u, 0u, 0u, 0u};
+  if (off + 16 <= r.w[2]) __builtin_memcpy(&v, (const void*)(base + off), 16);
+  return v;
+}
 
 }  // namespace emu
 
@@ -314,6 +323,49 @@ inline uint32_t cvt_pk_fp8_f32(float a, float b, uint32_t old, bool hi) {
   return hi ? (old & 0xffffu) | (v << 16) : (old & 0xffff0000u) | v;
 }
 }  // namespace emu
+namespace emu {
+typedef __attribute__((ext_vector_type(2))) _Float16 f16_pair;
+inline f16_pair cvt_pk_f16_fp8(uint32_t w, float scale, bool hi) {
+  w >>= hi ? 16 : 0;
+  f16_pair r;
+  r[0] = (_Float16)(e4m3_value(w & 255) * scale);
+  r[1] = (_Float16)(e4m3_value((w >> 8) & 255) * scale);
+  return r;
+}
+// v_perm_b32: bytes 0-3 are the second source's, 4-7 the first's
+inline uint32_t perm(uint32_t s0, uint32_t s1, uint32_t sel) {
+  const uint64_t both = ((uint64_t)s0 << 32) | s1;
+  uint32_t r = 0;
+  for (int i = 0; i < 4; ++i) r |= (uint32_t)((both >> (8 * ((sel >> (8 * i)) & 7))) & 255) << (8 * i);
+  return r;
+}
+// the fp16 products: the lanes of the bf16 ones
+template <int R, class V8, class VC>
+__forceinline__ VC mfma_f16(V8 a, V8 b, VC c) {
+  struct In {
+    _Float16 a[8], b[8];
+  } in;
+  __builtin_memcpy(in.a, &a, 16);
+  __builtin_memcpy(in.b, &b, 16);
+  const auto all = gather(in);
+  const int l = lane(), col = l % R;
+  VC d;
+  for (int r = 0; r < R * R / 64; ++r) {
+    const int row = R == 32 ? 8 * (r / 4) + 4 * (l / 32) + r % 4 : 4 * (l / 16) + r;
+    double s = c[r];
+    for (int part = 0; part < 64 / R; ++part) {
+      const In x = all[row + R * part], y = all[col + R * part];
+      for (int j = 0; j < 8; ++j) s += (double)(float)x.a[j] * (double)(float)y.b[j];
+    }
+    d[r] = (float)s;
+  }
+  return d;
+}
+}  // namespace emu
+#define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, hi) emu::cvt_pk_f16_fp8((w), (s), (hi))
+#define __builtin_amdgcn_perm(a, b, sel) emu::perm((a), (b), (sel))
+#define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) emu::mfma_f16<32>((a), (b), (c))
+#define __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, x, y, z) emu::mfma_f16<16>((a), (b), (c))
 #define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, hi) emu::cvt_pk_bf16_fp8((w), (s), (hi))
 #define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, hi) emu::cvt_pk_fp8_f32((a), (b), (old), (hi))
 #define __builtin_amdgcn_sinf(x) ((float)sin(2 * M_PI * (double)(x)))
@@ -339,6 +391,7 @@ inline void __threadfence() { std::atomic_thread_fence(std::memory_order_seq_cst
 #define __builtin_amdgcn_global_load_lds(g, l, size, off, aux) \
   emu::global_load_lds((const void*)(g), (const void*)(l), (size), (off))
 #define __builtin_amdgcn_make_buffer_rsrc(p, stride, num, flags) emu::make_rsrc((p), (stride), (num), (flags))
+#define __builtin_amdgcn_raw_buffer_load_b128(r, vo, so, aux) emu::raw_buffer_load_b128((r), (vo), (so))
 #define __builtin_amdgcn_raw_buffer_store_b128(v, r, vo, so, aux) emu::raw_buffer_store((v), (r), (vo), (so))
 #define __builtin_amdgcn_raw_buffer_store_b32(v, r, vo, so, aux) emu::raw_buffer_store((v), (r), (vo), (so))
 typedef emu::rsrc_t __amdgpu_buffer_rsrc_t;
