@@ -142,22 +142,34 @@ struct AppendArgs {
   const int32_t* start;
 };
 
+// x / s to the nearest, for |x / s| of at least 2^-11 and s of at least 2^-90 (else only near: what is below rounds to
+// code 0 all the same).  With inv = 1 / s to the nearest a faithful quotient corrected by its exact residual
+// is the nearest one (Markstein); the first correction makes it faithful.  5 operations to the division's 10 and more.
+__device__ __forceinline__ float quotient(float x, float s, float inv) {
+  float q = x * inv;
+  q = __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
+  return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
+}
+
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
+
 // A block of the grid takes a block of 64 tokens (and every gridDim.x-th after it) of one
-// (sequence, head), keys then values: its rows into registers, the largest
-// magnitude over the block, the codes out; the values' codes turn through LDS.  The last of a
-// (sequence, head)'s grid blocks to end moves the length on, so that none reads a moved one.
+// (sequence, head): its rows into registers, the largest magnitudes of the keys and of the values over the block, the
+// codes out.  A thread holds PASSES consecutive rows of 8 columns, so its codes of a key row are 8 bytes of it and
+// those of a value column PASSES bytes of that; the values' turn through LDS only to leave in whole rows of
+// [dim][64].  The last of a (sequence, head)'s grid blocks to end moves the length on, so that none reads a moved one.
 template <int D, int FMT>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int CH = D / 8;             // 16-byte pieces of a row
-  constexpr int RP = 256 / CH;          // rows of one pass of the threads
-  constexpr int PASSES = KB / RP;
+  constexpr int PASSES = KB * CH / 256; // consecutive rows of a thread: 4 or 8
+  constexpr int LD = KB + 16;           // bytes of a value column in LDS: 16-byte pieces stay aligned
   constexpr float CODE_MAX = FMT == SBSA_CACHE8_E4M3 ? 448.f : 127.f;
   const sbsa_cache8& c = a.c;
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
   const int64_t sh = (int64_t)s * c.num_kv_heads + h;
   const int64_t heads = (int64_t)c.num_seqs * c.num_kv_heads;
-  __shared__ float red[4];
-  __shared__ uint32_t turn[D * (KB / 4 + 1)];
+  __shared__ int red[2][4];
+  __shared__ __attribute__((aligned(16))) unsigned char turn[D * LD];
   __shared__ int s_last;
 
   int64_t row0;
@@ -174,86 +186,116 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const bool grows = end > start;
   const int first = start / KB, last = grows ? (end - 1) / KB : first - 1;
 
-  const int col = (tid % CH) * 8, r0 = tid / CH;
+  const int col = (tid % CH) * 8, r0 = tid / CH * PASSES;
+  const bf16_t* src[2] = {a.k + row0 * a.k_st + h * a.k_sh, a.v + row0 * a.v_st + h * a.v_sh};
+  const int64_t st[2] = {a.k_st, a.v_st};
+  bf16_t* const tail = (bf16_t*)c.tail + sh * KB * D;
+  const int64_t tail_v = heads * KB * D, scale_v = heads * c.num_blocks;
   for (int b = first + (int)blockIdx.x; b <= last; b += (int)gridDim.x) {
     const int64_t place = place_of(c, sh, b);
-#pragma unroll 1
-    for (int t = 0; t < 2; ++t) {
-      const bf16_t* src = t ? a.v + row0 * a.v_st + h * a.v_sh : a.k + row0 * a.k_st + h * a.k_sh;
-      const int64_t st = t ? a.v_st : a.k_st;
-      bf16_t* tail = (bf16_t*)c.tail + ((int64_t)t * heads + sh) * KB * D;
-      const float old_scale = c.scales[(int64_t)t * heads * c.num_blocks + place];
-      uint8_t* codes = t ? (uint8_t*)c.codes_v + place * KB * D : (uint8_t*)c.codes_k + place * KB * D;
-      u32x4_t x[PASSES];
-      float most = 0.f;
-      bool fine = true;
+    uint8_t* const codes[2] = {(uint8_t*)c.codes_k + place * KB * D, (uint8_t*)c.codes_v + place * KB * D};
+    u32x4_t x[2][PASSES];
+    const bool fresh = b * KB >= start && (b + 1) * KB <= end;     // the block is new rows throughout
+    if (fresh) {
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p) {
-        const int j = p * RP + r0, pos = b * KB + j;
-        u32x4_t w = {0u, 0u, 0u, 0u};
-        if (pos >= start && pos < end) {
-          w = *reinterpret_cast<const u32x4_t*>(src + (int64_t)(pos - start) * st + col);
-        } else if (pos < start && open == b) {
-          w = *reinterpret_cast<const u32x4_t*>(tail + (int64_t)j * D + col);
-        } else if (pos < start) {
-          // the row is there in its codes alone
-          bf16_t y[8];
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            y[i] = f2bf(decode1<FMT>(codes[t ? (col + i) * KB + j : j * D + col + i]) * old_scale);
-          __builtin_memcpy(&w, y, 16);
+        for (int p = 0; p < PASSES; ++p)
+          x[t][p] = *reinterpret_cast<const u32x4_t*>(src[t] + (int64_t)(b * KB + r0 + p - start) * st[t] + col);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+          const int j = r0 + p, pos = b * KB + j;
+          u32x4_t w = {0u, 0u, 0u, 0u};
+          if (pos >= start && pos < end) {
+            w = *reinterpret_cast<const u32x4_t*>(src[t] + (int64_t)(pos - start) * st[t] + col);
+          } else if (pos < start && open == b) {
+            w = *reinterpret_cast<const u32x4_t*>(tail + t * tail_v + j * D + col);
+          } else if (pos < start) {
+            // the row is there in its codes alone
+            const float old = c.scales[t * scale_v + place];
+            bf16_t y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              y[i] = f2bf(decode1<FMT>(codes[t][t ? (col + i) * KB + j : j * D + col + i]) * old);
+            __builtin_memcpy(&w, y, 16);
+          }
+          x[t][p] = w;
         }
-        x[p] = w;
-        bf16_t y[8];
-        __builtin_memcpy(y, &w, 16);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          fine = fine && (y[i] & 0x7f80) != 0x7f80;
-          most = fmaxf(most, fabsf(bf2f(y[i])));
-        }
-      }
-      // the block's largest magnitude; one value that is not finite makes the scale NaN
-      most = fine ? most : INFINITY;
-      most = wave_max(most);
-      __syncthreads();                  // every row is read before a code or the tail is written
-      if ((tid & 63) == 0) red[tid >> 6] = most;
-      __syncthreads();
-      most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-      fine = most < INFINITY;
-      const float scale = fine ? fmaxf(most / CODE_MAX, 0x1p-126f) : __uint_as_float(0x7fc00000u);
-      if (tid == 0) c.scales[(int64_t)t * heads * c.num_blocks + place] = scale;
-#pragma unroll
-      for (int p = 0; p < PASSES; ++p) {
-        const int j = p * RP + r0;
-        bf16_t y[8];
-        __builtin_memcpy(y, &x[p], 16);
-        uint32_t w[2] = {0u, 0u};
-        if (fine) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i >> 1] |= encode2<FMT>(bf2f(y[2 * i]) / scale, bf2f(y[2 * i + 1]) / scale) << (16 * (i & 1));
-        }
-        if (t == 0) {
-          u32x2_t o;
-          o.x = w[0]; o.y = w[1];
-          *reinterpret_cast<u32x2_t*>(codes + (int64_t)j * D + col) = o;
-        } else {
-          uint8_t* tb = reinterpret_cast<uint8_t*>(turn);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) tb[(col + i) * (KB + 4) + j] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
-        }
-        if (b == last && first == last) {
-          const int pos = b * KB + j;
-          if (pos < end && (pos >= start || open != b))
-            *reinterpret_cast<u32x4_t*>(tail + (int64_t)j * D + col) = x[p];
-        }
-      }
-      if (t == 1) {
-        __syncthreads();
-        for (int i = tid; i < D * (KB / 4); i += 256)
-          reinterpret_cast<uint32_t*>(codes)[i] = turn[(i / (KB / 4)) * (KB / 4 + 1) + i % (KB / 4)];
-      }
     }
+    // the largest magnitudes, as bf16 bits without the sign: those that are not finite are 0x7f80 and up
+    float scale[2];
+    bool fine[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      u16x2_t most = {0, 0};
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = x[t][p][i] & 0x7fff7fffu;
+          u16x2_t v;
+          __builtin_memcpy(&v, &w, 4);
+          most = __builtin_elementwise_max(most, v);
+        }
+      int m = most.x > most.y ? most.x : most.y;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
+      if ((tid & 63) == 0) red[t][tid >> 6] = m;
+    }
+    __syncthreads();                    // and every row is read before a code or the tail is written
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int m = max(max(red[t][0], red[t][1]), max(red[t][2], red[t][3]));
+      fine[t] = m < 0x7f80;
+      scale[t] = fine[t] ? fmaxf(bf2f((bf16_t)m) / CODE_MAX, 0x1p-126f) : __uint_as_float(0x7fc00000u);
+      if (tid == 0) c.scales[t * scale_v + place] = scale[t];
+    }
+    const bool easy = scale[0] >= 0x1p-90f && scale[1] >= 0x1p-90f;      // (no, where one is NaN)
+    const float inv[2] = {1.f / scale[0], 1.f / scale[1]};
+    auto value = [&](int t, int p, int i) {
+      const uint32_t w = x[t][p][i >> 1];
+      const float v = bf2f((bf16_t)(i & 1 ? w >> 16 : w & 0xffffu));
+      return easy ? quotient(v, scale[t], inv[t]) : v / scale[t];
+    };
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      uint32_t w[2] = {0u, 0u};
+      if (fine[0]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i >> 1] |= encode2<FMT>(value(0, p, 2 * i), value(0, p, 2 * i + 1)) << (16 * (i & 1));
+      }
+      u32x2_t o;
+      o.x = w[0]; o.y = w[1];
+      *reinterpret_cast<u32x2_t*>(codes[0] + (r0 + p) * D + col) = o;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t w[PASSES / 4];
+#pragma unroll
+      for (int x4 = 0; x4 < PASSES / 4; ++x4)
+        w[x4] = fine[1] ? encode2<FMT>(value(1, 4 * x4, i), value(1, 4 * x4 + 1, i)) |
+                              encode2<FMT>(value(1, 4 * x4 + 2, i), value(1, 4 * x4 + 3, i)) << 16
+                        : 0u;
+      __builtin_memcpy(turn + (col + i) * LD + r0, w, PASSES);
+    }
+    if (b == last && first == last) {
+      // the rows are kept: those that were the tail's already are there
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+          const int pos = b * KB + r0 + p;
+          if (pos < end && (pos >= start || open != b))
+            *reinterpret_cast<u32x4_t*>(tail + t * tail_v + (r0 + p) * D + col) = x[t][p];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = tid; i < D * (KB / 16); i += 256)
+      *reinterpret_cast<u32x4_t*>(codes[1] + i * 16) = *reinterpret_cast<const u32x4_t*>(turn + (i / 4) * LD + (i % 4) * 16);
     if (b * KB >= start && tid == 0) c.weights[sh * c.num_blocks + b] = 0.f;
     __syncthreads();                    // LDS is used again
   }
@@ -267,14 +309,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     if (!s_last) return;
     if (tid == 0) c.counters[sh] = 0;
     // the last block's rows are kept: all of them are new where it is not the first
-    for (int t = 0; t < 2 && last > first; ++t) {
-      const bf16_t* src = t ? a.v + row0 * a.v_st + h * a.v_sh : a.k + row0 * a.k_st + h * a.k_sh;
-      const int64_t st = t ? a.v_st : a.k_st;
-      bf16_t* tail = (bf16_t*)c.tail + ((int64_t)t * heads + sh) * KB * D;
-      for (int j = r0; last * KB + j < end && j < KB; j += RP)
-        *reinterpret_cast<u32x4_t*>(tail + (int64_t)j * D + col) =
-            *reinterpret_cast<const u32x4_t*>(src + (int64_t)(last * KB + j - start) * st + col);
-    }
+    for (int t = 0; t < 2 && last > first; ++t)
+      for (int j = r0; j < r0 + PASSES && last * KB + j < end; ++j)
+        *reinterpret_cast<u32x4_t*>(tail + t * tail_v + j * D + col) =
+            *reinterpret_cast<const u32x4_t*>(src[t] + (int64_t)(last * KB + j - start) * st[t] + col);
   }
   if (tid == 0) {
     c.lengths[sh] = end;
@@ -903,27 +941,20 @@ struct EvictArgs {
 
 constexpr int EVICT_THREADS = 1024;
 
-// Sum of a value over the block; `part` has a place per wave and is read by all afterwards.
-__device__ __forceinline__ int block_sum(int v, int* part) {
-  v = wave_sum_i32(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  int t = 0;
-  for (int i = 0; i < EVICT_THREADS / 64; ++i) t += part[i];
-  return t;
-}
-
-// One (sequence, head): tables into LDS whole (the outputs may be the inputs), the weight of the last block
-// that stays found bit by bit over the weights' bits (not negative, so their order is that of the
-// numbers), then every block's new place by a prefix sum over the threads' runs of blocks.
+// One (sequence, head): tables into LDS whole (the outputs may be the inputs); the weight of the last block that
+// stays by three histograms over its bits (not negative, so their order is that of the numbers), 11, 11
+// and 9 of them; then each wave counts its run of blocks, and writes it in order behind those before.
 __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
+  constexpr int BINS = 2048, WAVES = EVICT_THREADS / 64;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_evict[];
   int32_t* tab = reinterpret_cast<int32_t*>(smem_evict);
   uint32_t* bits = reinterpret_cast<uint32_t*>(tab + a.num_blocks);
-  __shared__ int part[EVICT_THREADS / 64];
+  __shared__ int hist[BINS];
+  __shared__ int part[WAVES], part_eq[WAVES];
+  __shared__ int s_bin[2];
   const int64_t sh = blockIdx.x, base = sh * a.num_blocks;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int room = a.num_blocks;
   int len = a.lengths[sh];
   len = len < 0 ? 0 : (len < room * KB ? len : room * KB);
@@ -933,68 +964,101 @@ __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
     tab[i] = a.table[base + i];
     bits[i] = __float_as_uint(a.weights[base + i]);
   }
-  __syncthreads();
-  const int stay = n < a.keep ? n : a.keep;
-  const int mid0 = a.sink < n ? a.sink : n, mid1 = n - a.recent > mid0 ? n - a.recent : mid0;
-  const int wanted = n > a.keep ? a.keep - a.sink - a.recent : mid1 - mid0;
+  const bool cuts = n > a.keep;
+  const int stay = cuts ? a.keep : n;
+  const int mid0 = a.sink, mid1 = n - a.recent;       // used where the sequence is cut
   auto key = [&](int i) -> uint32_t {
-    const float w = __uint_as_float(bits[i]);
-    return w > 0.f ? __float_as_uint(w) : 0u;
+    const uint32_t b = bits[i];
+    return __uint_as_float(b) > 0.f ? b : 0u;
   };
-  // the largest bound that at least `wanted` of the middle blocks reach
+  // bound: the key of the last of the heaviest `wanted` of the middle; above: how many are heavier
   uint32_t bound = 0;
-  int above = 0;                      // of them, strictly above the bound
-  if (n > a.keep) {
-    for (int bit = 30; bit >= 0; --bit) {
-      const uint32_t cand = bound | (1u << bit);
-      int v = 0;
-      for (int i = mid0 + tid; i < mid1; i += EVICT_THREADS) v += key(i) >= cand;
-      if (block_sum(v, part) >= wanted) bound = cand;
+  int above = 0;
+  const int wanted = a.keep - a.sink - a.recent;
+  if (cuts && wanted > 0) {
+    constexpr int SHIFT[3] = {20, 9, 0}, WIDTH[3] = {11, 11, 9};
+#pragma unroll
+    for (int round = 0; round < 3; ++round) {
+      hist[tid] = 0;
+      hist[tid + EVICT_THREADS] = 0;
+      __syncthreads();
+      for (int i = mid0 + tid; i < mid1; i += EVICT_THREADS) {
+        const uint32_t k = key(i);
+        if (round == 0 || k >> (SHIFT[round] + WIDTH[round]) == bound >> (SHIFT[round] + WIDTH[round]))
+          atomicAdd(&hist[(k >> SHIFT[round]) & ((1u << WIDTH[round]) - 1)], 1);
+      }
+      __syncthreads();
+      // keys in bins above this thread's pair, from the top: threads in reverse order
+      const int hi = BINS - 1 - 2 * tid;
+      const int h1 = hist[hi], h0 = hist[hi - 1];
+      const int incl = wave_incl_scan(h1 + h0);
+      if (lane == 63) part[wave] = incl;
+      __syncthreads();
+      int before = above + incl - h1 - h0;
+      for (int i = 0; i < wave; ++i) before += part[i];
+      if (before < wanted && before + h1 >= wanted) {
+        s_bin[0] = hi;
+        s_bin[1] = before;
+      } else if (before + h1 < wanted && before + h1 + h0 >= wanted) {
+        s_bin[0] = hi - 1;
+        s_bin[1] = before + h1;
+      }
+      __syncthreads();
+      bound |= (uint32_t)s_bin[0] << SHIFT[round];
+      above = s_bin[1];
     }
-    int v = 0;
-    for (int i = mid0 + tid; i < mid1; i += EVICT_THREADS) v += key(i) > bound;
-    above = block_sum(v, part);
+  } else if (cuts) {
+    bound = 0xffffffffu;                              // none of the middle stays
   }
-  const int ties = wanted - above;    // of those at the bound, the first that stay
-  // this thread's run of blocks
-  const int per = (room + EVICT_THREADS - 1) / EVICT_THREADS;
-  const int i0 = tid * per < room ? tid * per : room, i1 = i0 + per < room ? i0 + per : room;
-  auto prefix = [&](int v) {          // sum over the threads before this one
-    const int incl = wave_incl_scan(v);
-    __syncthreads();
-    if ((tid & 63) == 63) part[tid >> 6] = incl;
-    __syncthreads();
-    int t = incl - v;
-    for (int i = 0; i < (tid >> 6); ++i) t += part[i];
-    return t;
-  };
-  int eq = 0;
-  for (int i = i0; i < i1; ++i) eq += n > a.keep && i >= mid0 && i < mid1 && key(i) == bound;
-  const int eq_before = prefix(eq);
-  auto stays = [&](int i, int& seen) {
+  const int ties = wanted - above;                    // of those at the bound, the first that stay
+  __syncthreads();
+  // this wave's run of blocks: how many stay for sure, and how many are at the bound
+  const int run = (room + WAVES * 64 - 1) / (WAVES * 64) * 64;
+  const int i0 = wave * run, i1 = min(i0 + run, room);
+  auto sure = [&](int i, bool& at_bound) {
+    at_bound = false;
     if (i >= n) return false;
-    if (n <= a.keep || i < mid0 || i >= mid1) return true;
+    if (!cuts || i < mid0 || i >= mid1) return true;
     const uint32_t k = key(i);
-    if (k == bound) return seen++ < ties;
+    at_bound = k == bound;
     return k > bound;
   };
-  int kept = 0, seen = eq_before;
-  for (int i = i0; i < i1; ++i) kept += stays(i, seen);
-  int at = prefix(kept);
-  seen = eq_before;
-  for (int i = i0; i < i1; ++i) {
-    int to = i;
-    float w = 0.f;
-    const bool here = stays(i, seen);
-    if (here) {
-      to = at++;
-      w = __uint_as_float(bits[i]);
-    } else if (i < n) {
-      to = stay + i - at;             // behind those that stay: of the i blocks before, `at` stayed
+  int kept = 0, eq = 0;
+  for (int i = i0; i < i1; i += 64) {
+    bool at_bound = false;
+    const bool yes = i + lane < i1 && sure(i + lane, at_bound);
+    kept += __popcll(__ballot(yes));
+    eq += __popcll(__ballot(i + lane < i1 && at_bound));
+  }
+  if (lane == 0) {
+    part[wave] = kept;
+    part_eq[wave] = eq;
+  }
+  __syncthreads();
+  int at = 0, seen = 0;
+  for (int w = 0; w < wave; ++w) {
+    at += part[w];
+    seen += part_eq[w];
+  }
+  at += min(seen, max(ties, 0));                      // of the ties before, those that stay
+  const unsigned long long below = (1ull << lane) - 1;
+  for (int i = i0; i < i1; i += 64) {
+    const int b = i + lane;
+    bool at_bound = false;
+    bool here = b < i1 && sure(b, at_bound);
+    at_bound = at_bound && b < i1;
+    const unsigned long long tied = __ballot(at_bound);
+    here = here || (at_bound && seen + __popcll(tied & below) < ties);
+    const unsigned long long all = __ballot(here);
+    const int before = at + __popcll(all & below);    // blocks that stay before this one
+    if (b < i1) {
+      const int to = here ? before : (b < n ? stay + b - before : b);
+      a.table_out[base + to] = tab[b];
+      a.weights_out[base + to] = here ? __uint_as_float(bits[b]) : 0.f;
+      if (b == open) a.open_out[sh] = here ? to : -1;
     }
-    a.table_out[base + to] = tab[i];
-    a.weights_out[base + to] = w;
-    if (i == open) a.open_out[sh] = here ? to : -1;
+    at += __popcll(all);
+    seen += __popcll(tied);
   }
   if (tid == 0) {
     a.lengths_out[sh] = len - (n - stay) * KB;

@@ -4,9 +4,10 @@
 // turn in 64-bit fixed point: position x turns mod 2^64 loses nothing at any position (in
 // fp32 the angle of position 10^6 would be off by 0.06), and the sine unit takes turns.
 //
-// A block takes one token (and a share of its heads): thread (unit, head) holds the sines
-// of its VEC pairs in registers and loops over heads, so they are made once for a
-// token and 1/HL of its heads.  A unit is VEC pairs (two vectors of VEC values), or VEC values that pass.
+// A thread takes a unit (VEC pairs: two vectors of VEC values; or VEC values that pass) of one token in
+// HEADS heads, every HEADS-th group of them to a thread: the sines of its pairs are made once for HEADS heads, and its
+// loads are all on their way before the first is used.  The work is a row of items over all threads, so
+// that no thread is left over whatever the head count and the rotated share.
 #include "sbsa_common.h"
 
 namespace {
@@ -23,7 +24,8 @@ struct RotaryArgs {
   const uint8_t* axes;
   float gain;
   int pos_bytes, inverse;
-  int hq, hkv, rotary_dim, units, rot_units, unit_lanes, head_lanes;
+  int hq, hkv, rotary_dim, units, rot_units, groups;
+  uint32_t items;
 };
 
 template <int VEC>
@@ -54,65 +56,60 @@ __device__ __forceinline__ void store_vec(bf16_t* p, const bf16_t (&x)[VEC]) {
   }
 }
 
-template <int VEC, bool INTERLEAVED>
+template <int VEC, bool INTERLEAVED, int HEADS>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-  const int64_t tok = blockIdx.x;
-  const int unit0 = threadIdx.x % a.unit_lanes;
-  const int hl = threadIdx.x / a.unit_lanes;
-  if (hl >= a.head_lanes) return;
-  const int heads = a.hq + a.hkv;
-  const int head_step = a.head_lanes * gridDim.y;
-  for (int u = unit0; u < a.units; u += a.unit_lanes) {
-    const bool rot = u < a.rot_units;
-    float c[VEC], s[VEC];
-    // the two vectors' places: (i, i + rotary_dim/2), neighbours, or one that passes
-    int d0, d1;
-    if (rot) {
-      d0 = INTERLEAVED ? 2 * VEC * u : VEC * u;
-      d1 = INTERLEAVED ? d0 + VEC : d0 + a.rotary_dim / 2;
+  // item = (token, group of heads, unit)
+  const uint32_t item = blockIdx.x * 256u + threadIdx.x;
+  if (item >= a.items) return;
+  const uint32_t row = item / (uint32_t)a.units, u = item - row * (uint32_t)a.units;
+  const int64_t tok = row / (uint32_t)a.groups;
+  const int group = (int)(row - (uint32_t)tok * (uint32_t)a.groups);
+  const bool rot = (int)u < a.rot_units;
+  // the two vectors' places: (i, i + rotary_dim/2), neighbours, or one that passes
+  const int d0 = rot ? (INTERLEAVED ? 2 * VEC * (int)u : VEC * (int)u) : a.rotary_dim + VEC * ((int)u - a.rot_units);
+  const int d1 = INTERLEAVED ? d0 + VEC : d0 + a.rotary_dim / 2;
+  bf16_t x[HEADS][VEC], y[HEADS][VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int pair = VEC * u + i;
-        const int64_t at = (a.axes ? (int64_t)a.axes[pair] * a.pos_axis : 0) + tok * a.pos_stride;
-        const int64_t pos = a.pos_bytes == 8 ? reinterpret_cast<const int64_t*>(a.positions)[at]
-                                             : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[at];
-        const uint64_t angle = (uint64_t)pos * a.turns[pair];
-        const float t = (float)(int32_t)(angle >> 32) * 0x1p-32f;      // in [-1/2, 1/2] turns
-        c[i] = __builtin_amdgcn_cosf(t) * a.gain;
-        s[i] = __builtin_amdgcn_sinf(a.inverse ? -t : t) * a.gain;
-      }
-    } else {
-      d0 = d1 = a.rotary_dim + VEC * (u - a.rot_units);
+  for (int j = 0; j < HEADS; ++j) {
+    const int h = group + j * a.groups;
+    if (h < a.hq + a.hkv) {
+      const bf16_t* in = h < a.hq ? a.q + tok * a.q_st + h * a.q_sh : a.k + tok * a.k_st + (h - a.hq) * a.k_sh;
+      load_vec<VEC>(in + d0, x[j]);
+      if (rot) load_vec<VEC>(in + d1, y[j]);
     }
-    for (int h = blockIdx.y * a.head_lanes + hl; h < heads; h += head_step) {
-      const bool is_q = h < a.hq;
-      const int hh = is_q ? h : h - a.hq;
-      const bf16_t* in = is_q ? a.q + tok * a.q_st + hh * a.q_sh : a.k + tok * a.k_st + hh * a.k_sh;
-      bf16_t* out = is_q ? a.qo + tok * a.qo_st + hh * a.qo_sh : a.ko + tok * a.ko_st + hh * a.ko_sh;
-      bf16_t x[VEC], y[VEC];
-      load_vec<VEC>(in + d0, x);
-      if (!rot) {
-        store_vec<VEC>(out + d0, x);
-        continue;
-      }
-      load_vec<VEC>(in + d1, y);
-      // x, y: first and second members where the pairs are apart, 2 VEC neighbours otherwise
+  }
+  float c[VEC], s[VEC];
+  if (rot) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if constexpr (INTERLEAVED) {
-          bf16_t& pa = 2 * i < VEC ? x[2 * i] : y[2 * i - VEC];
-          bf16_t& pb = 2 * i + 1 < VEC ? x[2 * i + 1] : y[2 * i + 1 - VEC];
+    for (int i = 0; i < VEC; ++i) {
+      const int pair = VEC * (int)u + i;
+      const int64_t at = (a.axes ? (int64_t)a.axes[pair] * a.pos_axis : 0) + tok * a.pos_stride;
+      const int64_t pos = a.pos_bytes == 8 ? reinterpret_cast<const int64_t*>(a.positions)[at]
+                                           : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[at];
+      const uint64_t angle = (uint64_t)pos * a.turns[pair];
+      const float t = (float)(int32_t)(angle >> 32) * 0x1p-32f;      // in [-1/2, 1/2] turns
+      c[i] = __builtin_amdgcn_cosf(t) * a.gain;
+      s[i] = __builtin_amdgcn_sinf(a.inverse ? -t : t) * a.gain;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j) {
+    const int h = group + j * a.groups;
+    if (h < a.hq + a.hkv) {
+      bf16_t* out = h < a.hq ? a.qo + tok * a.qo_st + h * a.qo_sh : a.ko + tok * a.ko_st + (h - a.hq) * a.ko_sh;
+      if (rot) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          // where the pairs are neighbours, x and y are 2 VEC values in a row
+          bf16_t& pa = !INTERLEAVED ? x[j][i] : 2 * i < VEC ? x[j][(2 * i) % VEC] : y[j][(2 * i) % VEC];
+          bf16_t& pb = !INTERLEAVED ? y[j][i] : 2 * i + 1 < VEC ? x[j][(2 * i + 1) % VEC] : y[j][(2 * i + 1) % VEC];
           const float fa = bf2f(pa), fb = bf2f(pb);
           pa = f2bf(fa * c[i] - fb * s[i]);
           pb = f2bf(fb * c[i] + fa * s[i]);
-        } else {
-          const float fa = bf2f(x[i]), fb = bf2f(y[i]);
-          x[i] = f2bf(fa * c[i] - fb * s[i]);
-          y[i] = f2bf(fb * c[i] + fa * s[i]);
         }
+        store_vec<VEC>(out + d1, y[j]);
       }
-      store_vec<VEC>(out + d0, x);
-      store_vec<VEC>(out + d1, y);
+      store_vec<VEC>(out + d0, x[j]);
     }
   }
 }
@@ -121,24 +118,31 @@ bool aligned(const void* p, int64_t st, int64_t sh, int vec) {
   return ((uintptr_t)p % (2 * vec)) == 0 && st % vec == 0 && sh % vec == 0;
 }
 
+template <int VEC, int HEADS>
+void launch_heads(RotaryArgs a, int64_t rows, int interleaved, hipStream_t stream) {
+  a.groups = (a.hq + a.hkv + HEADS - 1) / HEADS;
+  a.items = (uint32_t)(rows * a.groups);
+  const dim3 grid((a.items + 255) / 256);
+  if (interleaved)
+    hipLaunchKernelGGL((rotary_kernel<VEC, true, HEADS>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((rotary_kernel<VEC, false, HEADS>), grid, dim3(256), 0, stream, a);
+}
+
+// False: more items than 32 bits count.
 template <int VEC>
-void launch_rotary(RotaryArgs a, int64_t tokens, int head_dim, bool in_place, int interleaved, hipStream_t stream) {
+bool launch_rotary(RotaryArgs a, int64_t tokens, int head_dim, bool in_place, int interleaved, hipStream_t stream) {
   a.rot_units = a.rotary_dim / (2 * VEC);
   // what passes is there already where the outputs are the inputs
   a.units = a.rot_units + (in_place ? 0 : (head_dim - a.rotary_dim) / VEC);
-  a.unit_lanes = a.units < 256 ? a.units : 256;
-  a.head_lanes = 256 / a.unit_lanes;
-  const int heads = a.hq + a.hkv;
-  if (a.head_lanes > heads) a.head_lanes = heads;
-  // few tokens: the heads over more blocks, until the blocks fill the card
-  int shares = (heads + a.head_lanes - 1) / a.head_lanes;
-  const int64_t most = 512 / tokens;
-  if (shares > most) shares = most < 1 ? 1 : (int)most;
-  const dim3 grid((unsigned)tokens, (unsigned)shares);
-  if (interleaved)
-    hipLaunchKernelGGL((rotary_kernel<VEC, true>), grid, dim3(256), 0, stream, a);
+  const int64_t rows = tokens * a.units;
+  if (rows * (a.hq + a.hkv) >= (1ll << 32) - 256) return false;
+  // a thread per head until there are threads for half of the card's 524288 places, then four heads to each
+  if (rows * (a.hq + a.hkv) <= 262144)
+    launch_heads<VEC, 1>(a, rows, interleaved, stream);
   else
-    hipLaunchKernelGGL((rotary_kernel<VEC, false>), grid, dim3(256), 0, stream, a);
+    launch_heads<VEC, 4>(a, rows, interleaved, stream);
+  return true;
 }
 
 }  // namespace
@@ -169,12 +173,10 @@ extern "C" int sbsa_rotary(const void* q, int64_t q_st, int64_t q_sh, void* q_ou
            aligned(q_out, qo_st, qo_sh, vec) &&
            (num_kv_heads == 0 || (aligned(k, k_st, k_sh, vec) && aligned(k_out, ko_st, ko_sh, vec)));
   };
-  if (fits(8))
-    launch_rotary<8>(a, tokens, head_dim, in_place, interleaved, stream);
-  else if (fits(2))
-    launch_rotary<2>(a, tokens, head_dim, in_place, interleaved, stream);
-  else
-    launch_rotary<1>(a, tokens, head_dim, in_place, interleaved, stream);
+  const bool ok = fits(8)   ? launch_rotary<8>(a, tokens, head_dim, in_place, interleaved, stream)
+                  : fits(2) ? launch_rotary<2>(a, tokens, head_dim, in_place, interleaved, stream)
+                            : launch_rotary<1>(a, tokens, head_dim, in_place, interleaved, stream);
+  if (!ok) return SBSA_ERR_UNSUPPORTED;
   SBSA_CHECK_LAUNCH();
   return SBSA_OK;
 }

@@ -81,11 +81,12 @@ class SembloAttention:
         # test hook: a list here receives every sparse chunk's selection (ChunkPlan.record)
         self.plan_log: list | None = None
         self._projections = None
+        self._rotary = None
         self._capacity_arena: DecodeArena | None = None
         register_layer(self.layer_name, self)
 
     # -- the model's projections (attached by the caller) -------------------------
-    def attach_projections(self, project_qkv, finish_output, project_kv=None) -> None:
+    def attach_projections(self, project_qkv, finish_output, project_kv=None, rotary=None) -> None:
         """The model's side of the layer, for the sessions driven by hidden states.
 
         ``project_qkv(rope_positions, hidden_states)`` returns (q_post, k_post, v,
@@ -94,8 +95,11 @@ class SembloAttention:
         qwen3_5_model.py:135, nemotron_h_model.py:149).  ``finish_output(attn, gate)``
         takes the attention [n, Hq*D] to the layer's output (``_finish_output``,
         qwen3_5_model.py:225-235).  ``project_kv`` returns (k_post, v, k_pre) alone; by
-        default the full projection runs and Q is dropped (model.py:356-368)."""
+        default the full projection runs and Q is dropped (model.py:356-368).
+        ``rotary`` (``rotary.RotaryEmbedding``): the projections then leave q_post and k_post None,
+        and the layer makes them from q_pre and k_pre at the rotary positions."""
         self._projections = (project_qkv, finish_output, project_kv)
+        self._rotary = rotary
 
     def _require_projections(self):
         if self._projections is None:
@@ -104,13 +108,21 @@ class SembloAttention:
         return self._projections
 
     def _project_qkv(self, rope_positions, hidden_states):
-        return self._require_projections()[0](rope_positions, hidden_states)
+        q_post, k_post, v, q_pre, k_pre, gate = self._require_projections()[0](rope_positions, hidden_states)
+        if self._rotary is not None and q_post is None and k_post is None:
+            n = hidden_states.shape[0]
+            q_post, k_post = self._rotary(rope_positions, q_pre.view(n, self.num_heads, self.head_dim),
+                                          k_pre.view(n, self.num_kv_heads, self.head_dim))
+        return q_post, k_post, v, q_pre, k_pre, gate
 
     def _project_kv(self, rope_positions, hidden_states):
         project_qkv, _, project_kv = self._require_projections()
         if project_kv is not None:
-            return project_kv(rope_positions, hidden_states)
-        _q, k_post, v, _qp, k_pre, _g = project_qkv(rope_positions, hidden_states)
+            k_post, v, k_pre = project_kv(rope_positions, hidden_states)
+        else:
+            _q, k_post, v, _qp, k_pre, _g = project_qkv(rope_positions, hidden_states)
+        if self._rotary is not None and k_post is None:
+            k_post = self._rotary(rope_positions, k_pre.view(hidden_states.shape[0], self.num_kv_heads, self.head_dim))
         return k_post, v, k_pre
 
     def _finish_output(self, attn: torch.Tensor, gate):
