@@ -470,7 +470,7 @@ int sbsa_rotary(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t 
 
 /* The cache of num_seqs sequences.  A block's place is table[seq, head, block], a permutation
  * of 0 .. num_blocks-1 for each (seq, head); entries outside are read as the nearest place.
- * A value is code x scale; a block that holds a value that is not finite has scale NaN.
+ * A value is code x scale; scales are positive, and NaN where a block holds a value that is not finite.
  * The codes behind a sequence's last token may hold anything. */
 typedef struct sbsa_cache8 {
   void* codes_k;        /* [S, Hkv, N, 64, dim] bytes, 16-byte aligned            */

@@ -16,6 +16,7 @@ constexpr float LN2 = 0.69314718055994530942f;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+typedef __attribute__((ext_vector_type(4))) int32_t i32x4_t;
 
 __device__ __forceinline__ f16x8_t as_f16x8(u32x4_t v) {
   f16x8_t r;
@@ -301,10 +302,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   }
 
   if (gridDim.x > 1) {
-    if (tid == 0) {
-      __threadfence();
-      s_last = atomicAdd(&c.counters[sh], 1) == (int)gridDim.x - 1;
-    }
+    // Every read of this block has ended (its values were used before the barrier above, or are by the next), so the
+    // ticket needs no fence: a release would write the XCD's L2 back, 2000 times in a long prompt (133 us to 50).
+    __syncthreads();
+    if (tid == 0) s_last = atomicAdd(&c.counters[sh], 1) == (int)gridDim.x - 1;
     __syncthreads();
     if (!s_last) return;
     if (tid == 0) c.counters[sh] = 0;
@@ -329,46 +330,86 @@ struct AttendArgs {
   bf16_t* out;
   int64_t o_st, o_sh;
   float* lse;                  // [tokens, Hq], natural
-  float* part_o;               // [splits][tokens * Hq][D]
+  float* part_o;               // [Hkv][slots][tile rows][D]
   // Sums of exponentials are kept as (m, l), 2^m l: the logarithm of one would round a weight by 10^-6
-  f32x2_t* part_ml;            // [splits][tokens * Hq]
+  f32x2_t* part_ml;            // [Hkv][slots][tile rows]
+  i32x4_t* where;                 // [tokens * Hq]: a row's first slot, its slots, its place in the tile
   f32x2_t* row_ml;             // [tokens * Hq], with 1 / l (accumulating)
   f32x2_t* part_w;             // [tokens * Hq][N]: each block's sum of a row (few rows, accumulating)
   const int32_t* offsets;
   int64_t tokens, uniform;
-  int hq, g, splits, tile_queries, tiles_per_seq;
+  int hq, g, tile_queries, tile_rows, slots, target;
   float scale_log2;            // sm_scale * log2(e)
 };
 
-// The row tile of this block of the grid: sequence, its rows, and the tile's first query.  With
-// offsets the tiles are counted along the sequences, 64 of them at a time; false: no tile is left.
-__device__ __forceinline__ bool tile_of(const AttendArgs& a, int64_t t, int& s, int64_t& row0, int& n, int& q0) {
-  if (!a.offsets) {
-    s = (int)(t / a.tiles_per_seq);
-    rows_of(nullptr, s, a.uniform, a.tokens, row0, n);
-    q0 = (int)(t % a.tiles_per_seq) * a.tile_queries;
-    return true;
+// The share of a slot (grid block x): a tile of rows of one sequence, and a run of the blocks that it sees.
+struct Share {
+  int s, n, q0, held, lo, hi, first, count;
+  int64_t row0;
+};
+
+// The shares are equal runs of blocks over all tiles (target of them, or whole tiles where target is 0): a
+// long sequence gets more of them than a short one.  Every wave works its own out from the sequences' lengths, a lane to
+// a sequence, 64 sequences at a time.  False: the slot is left over.
+__device__ __forceinline__ bool share_of(const AttendArgs& a, int h, int slot, Share& x) {
+  const int lane = threadIdx.x & 63, seqs = a.c.num_seqs;
+  auto look = [&](int s, int64_t& row0, int& n, int& held, int& tiles, int& blocks) {
+    row0 = 0;
+    n = held = tiles = blocks = 0;
+    if (s < seqs) {
+      rows_of(a.offsets, s, a.uniform, a.tokens, row0, n);
+      held = held_of(a.c, (int64_t)s * a.c.num_kv_heads + h);
+      tiles = (n + a.tile_queries - 1) / a.tile_queries;
+      blocks = (held + KB - 1) / KB;
+    }
+  };
+  int64_t row0;
+  int n, held, tiles, blocks;
+  look(lane, row0, n, held, tiles, blocks);
+  int per = 0x7fffffff;
+  if (a.target) {
+    int total = tiles * blocks;
+    for (int s0 = 64; s0 < seqs; s0 += 64) {
+      int64_t r;
+      int m, e, t, b;
+      look(s0 + lane, r, m, e, t, b);
+      total += t * b;
+    }
+    total = wave_sum_i32(total);
+    per = (total + a.target - 1) / a.target;
+    per = per < 4 ? 4 : per;
   }
-  const int lane = threadIdx.x & 63;
-  int64_t before = 0;
-  for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64) {
-    int64_t r = 0;
-    int m = 0;
-    if (s0 + lane < a.c.num_seqs) rows_of(a.offsets, s0 + lane, 0, a.tokens, r, m);
-    const int mine = (m + a.tile_queries - 1) / a.tile_queries;
+  int before = 0;
+  for (int s0 = 0;; s0 += 64) {
+    const int shares = blocks <= per ? 1 : (blocks + per - 1) / per;
+    const int mine = tiles * shares;
     const int upto = wave_incl_scan(mine);
-    const unsigned long long past = __ballot(before + upto > t);
+    const unsigned long long past = __ballot(before + upto > slot);
     if (past) {
       const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)past) - 1);
-      s = s0 + l;
-      rows_of(a.offsets, s, 0, a.tokens, row0, n);
-      const int upto_l = __builtin_amdgcn_readlane(upto, l), mine_l = __builtin_amdgcn_readlane(mine, l);
-      q0 = (int)(t - before - (upto_l - mine_l)) * a.tile_queries;
+      x.s = s0 + l;
+      x.n = __builtin_amdgcn_readlane(n, l);
+      x.held = __builtin_amdgcn_readlane(held, l);
+      x.row0 = (int64_t)__builtin_amdgcn_readlane((int)row0, l);       // below 2^24
+      const int count = __builtin_amdgcn_readlane(shares, l);
+      const int own = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l);
+      const int tile = (slot - own) / count, part = (slot - own) - tile * count;
+      x.q0 = tile * a.tile_queries;
+      x.first = slot - part;
+      x.count = count;
+      // the blocks that the tile's last row sees, of which this is share `part`
+      const int last = x.q0 + a.tile_queries < x.n ? x.q0 + a.tile_queries : x.n;
+      const int sees = x.held - x.n + last;
+      const int all = sees > 0 ? (sees + KB - 1) / KB : 0;
+      const int each = (all + count - 1) / count;
+      x.lo = part * each;
+      x.hi = x.lo + each < all ? x.lo + each : all;
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
+    if (s0 + 64 >= seqs) return false;
+    look(s0 + 64 + lane, row0, n, held, tiles, blocks);
   }
-  return false;
 }
 
 // 16 codes, those from `keep` on as 0: what lies behind a sequence's last token may be any bits
@@ -592,60 +633,54 @@ struct WaveRows {
   // four consecutive dims of the lane's row: tile t, quarter x of the accumulator
   static __device__ __forceinline__ int dim_of(int t, int x, int lane) { return t * R + 8 * x + 4 * (lane / R); }
 
-  // where a row's result goes: out, or its share's partial row
-  static __device__ __forceinline__ void store(const AttendArgs& a, int split, int64_t token, int head, int t, int x,
-                                               int lane, f32x4_t v) {
-    if (a.splits == 1) {
-      u32x2_t w;
-      w.x = pack2bf(v.x, v.y);
-      w.y = pack2bf(v.z, v.w);
-      *reinterpret_cast<u32x2_t*>(a.out + token * a.o_st + head * a.o_sh + dim_of(t, x, lane)) = w;
-    } else {
-      const int64_t row = (split * a.tokens + token) * a.hq + head;
-      *reinterpret_cast<f32x4_t*>(a.part_o + row * D + dim_of(t, x, lane)) = v;
-    }
-  }
-  // m, l: a row without keys has l = 0
-  static __device__ __forceinline__ void store_sum(const AttendArgs& a, int split, int64_t token, int head, float m, float l) {
-    const int64_t row = token * a.hq + head;
-    if (a.splits > 1)
-      a.part_ml[split * a.tokens * a.hq + row] = f32x2_t{m, l};
-    else
-      finish_row(a, row, m, l);
-  }
 };
 
-// This lane's row of a tile, what it sees, and the tile's share of the blocks.
+// This lane's row of a tile, and what it sees.
 template <int R>
 struct LaneRow {
-  int qi, head, vis, vis_most, vis_least, lo, hi, held;
+  int r, head, vis, vis_most, vis_least;
   bool there;
-  int64_t sh;
+  int64_t token;
 
-  __device__ __forceinline__ void find(const AttendArgs& a, int s, int h, int n, int q0, int r, int split) {
-    sh = (int64_t)s * a.c.num_kv_heads + h;
-    held = __builtin_amdgcn_readfirstlane(held_of(a.c, sh));
-    qi = q0 + r / a.g;
+  __device__ __forceinline__ void find(const AttendArgs& a, int h, const Share& x, int row) {
+    r = row;
+    const int qi = x.q0 + r / a.g;
     head = h * a.g + r % a.g;
-    there = r < a.tile_queries * a.g && qi < n;
-    vis = there ? held - n + qi + 1 : 0;
+    there = r < a.tile_queries * a.g && qi < x.n;
+    token = x.row0 + qi;
+    vis = there ? x.held - x.n + qi + 1 : 0;
     vis = vis < 0 ? 0 : vis;
     vis_most = vis;
     vis_least = there ? vis : 0x7fffffff;
 #pragma unroll
-    for (int x = 1; x < R; x <<= 1) {
-      vis_most = max(vis_most, __shfl_xor(vis_most, x, 64));
-      vis_least = min(vis_least, __shfl_xor(vis_least, x, 64));
+    for (int y = 1; y < R; y <<= 1) {
+      vis_most = max(vis_most, __shfl_xor(vis_most, y, 64));
+      vis_least = min(vis_least, __shfl_xor(vis_least, y, 64));
     }
     vis_most = __builtin_amdgcn_readfirstlane(vis_most);
     vis_least = __builtin_amdgcn_readfirstlane(vis_least);
-    // the share: of the blocks that the tile's last row sees
-    const int tile_last = q0 + a.tile_queries < n ? q0 + a.tile_queries : n;
-    const int tile_vis = held - n + tile_last;
-    const int blocks = tile_vis > 0 ? (tile_vis + KB - 1) / KB : 0;
-    const int per = (blocks + a.splits - 1) / a.splits;
-    lo = split * per;
-    hi = lo + per < blocks ? lo + per : blocks;
+  }
+
+  // four dims of the row's result: to out, or where its shares are joined
+  __device__ __forceinline__ void store(const AttendArgs& a, int h, int slot, const Share& x, int D, int dim, f32x4_t v) const {
+    if (x.count == 1) {
+      u32x2_t w;
+      w.x = pack2bf(v.x, v.y);
+      w.y = pack2bf(v.z, v.w);
+      *reinterpret_cast<u32x2_t*>(a.out + token * a.o_st + head * a.o_sh + dim) = w;
+    } else {
+      const int64_t at = ((int64_t)h * a.slots + slot) * a.tile_rows + r;
+      *reinterpret_cast<f32x4_t*>(a.part_o + at * D + dim) = v;
+    }
+  }
+  // the row's sum, by one lane of it: without keys it has l = 0
+  __device__ __forceinline__ void store_sum(const AttendArgs& a, int h, int slot, const Share& x, float m, float l) const {
+    const int64_t row = token * a.hq + head;
+    if (a.target) {
+      if (slot == x.first) a.where[row] = i32x4_t{x.first, x.count, r, 0};
+      a.part_ml[((int64_t)h * a.slots + slot) * a.tile_rows + r] = f32x2_t{m, l};
+    }
+    if (x.count == 1) finish_row(a, row, m, l);
   }
 };
 
@@ -664,33 +699,30 @@ __global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_keys_
   const sbsa_cache8& c = a.c;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int split = (int)(blockIdx.x % a.splits);
-  const int64_t tiles = gridDim.x / a.splits;
-  int s, n, q0;
-  int64_t row0;
-  if (!tile_of(a, tiles - 1 - blockIdx.x / a.splits, s, row0, n, q0)) return;
+  const int h = blockIdx.y, slot = blockIdx.x;
+  Share sh;
+  if (!share_of(a, h, slot, sh)) return;
   LaneRow<R> r;
-  r.find(a, s, (int)blockIdx.y, n, q0, lane % R, split);
-  const int64_t token = row0 + r.qi;
-  const bf16_t* qrow = r.there ? a.q + token * a.q_st + r.head * a.q_sh : nullptr;
+  r.find(a, h, sh, lane % R);
+  const bf16_t* qrow = r.there ? a.q + r.token * a.q_st + r.head * a.q_sh : nullptr;
   for (int i = wave; i < PIECES; i += 4) sq[i * 64 + lane] = W::query_piece(qrow, i >> 1, i & 1, lane);
 
   W w;
   w.start();
   const int64_t heads = (int64_t)c.num_seqs * c.num_kv_heads;
-  const int64_t base = r.sh * c.num_blocks;
+  const int64_t row = (int64_t)sh.s * c.num_kv_heads + h, base = row * c.num_blocks;
   const uint8_t* codes_k = (const uint8_t*)c.codes_k + base * KB * D;
   const uint8_t* codes_v = (const uint8_t*)c.codes_v + base * KB * D;
-  const int first = r.lo + wave;
-  const int count = r.hi > first ? (r.hi - first + 3) / 4 : 0;
+  const int first = sh.lo + wave;
+  const int count = sh.hi > first ? (sh.hi - first + 3) / 4 : 0;
   // the places and scales of the wave's next 64 blocks, one per lane
   int place = 0;
   float ks = 0.f, vs = 0.f;
   auto fetch = [&](int i0) {
     const int b = first + 4 * (i0 + lane);
     place = 0;
-    if (b < r.hi) {
-      place = (int)(place_of(c, r.sh, b) - base);
+    if (b < sh.hi) {
+      place = (int)(place_of(c, row, b) - base);
       ks = c.scales[base + place] * a.scale_log2;
       vs = c.scales[heads * c.num_blocks + base + place];
     }
@@ -720,9 +752,9 @@ __global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_keys_
       if constexpr (R == 16) sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
       if (r.there && lane < R)
-        a.part_w[(token * a.hq + r.head) * c.num_blocks + b] = f32x2_t{w.m, sum};
+        a.part_w[(r.token * a.hq + r.head) * c.num_blocks + b] = f32x2_t{w.m, sum};
     }
-    w.values(vc, p, r.held - b * KB, lane);
+    w.values(vc, p, sh.held - b * KB, lane);
     if (i + 1 < count) W::load_v(codes_v + at, lane, vc);
     asm volatile("" ::: "memory");                  // the queries stay in LDS, not in registers
   }
@@ -760,125 +792,348 @@ __global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_keys_
         const int at = (t * W::NI + 4 * q + i) * 64 + lane;
         v[i] = (fold[at] * f[0] + fold[TILE + at] * f[1]) + (fold[2 * TILE + at] * f[2] + fold[3 * TILE + at] * f[3]);
       }
-      W::store(a, split, token, r.head, t, q, lane, v);
+      r.store(a, h, slot, sh, D, W::dim_of(t, q, lane), v);
     }
   }
-  if (wave == 0 && lane < R) W::store_sum(a, split, token, r.head, top, total);
+  if (wave == 0 && lane < R) r.store_sum(a, h, slot, sh, top, total);
 }
 
-// Many rows: 32 of them to each wave, over one share of the keys.
+// Many rows: 32 of them to each wave, the tiles of codes in LDS for all four.  The codes stay 8 bits wide there
+// (half the LDS traffic of bf16 tiles, which would keep LDS as busy as the matrix cores) and each wave decodes what it reads;
+// a block of keys is taken in two halves of 32, so that two grid blocks fit a compute unit's registers and one's
+// softmax runs under the other's products.
+//
+// LDS holds a block's tiles as 16-byte pieces, swizzled so that the 8 lanes of a read's cycle meet
+// different banks: piece c of key row r at c ^ key_swizzle(r), piece c of dim row d at c ^ (d / 2) % 4.  They come straight from
+// memory (loads into LDS), the next block's while this one is used.
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+// 16 bytes per lane from memory straight to LDS, lane l's at lds_addr + 16 l.  In assembly, because the compiler waits for
+// the builtin's loads before any LDS read that it cannot tell apart; the kernel waits (vmcnt) before the
+// barrier that publishes a tile.  M0 holds the LDS base; nothing else in the kernel uses it.
+__device__ __forceinline__ void lds_load16(u32x4_t rsrc, uint32_t lds_addr, uint32_t voffset) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_addr), "v"(voffset), "s"(rsrc)
+               : "memory", "m0");
+}
+
+// a value that is the same in every lane, in a scalar register
+__device__ __forceinline__ float uniform(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(v)));
+}
+
+// A load through the scalar cache, by an address that is the same in every lane (of memory that no block of the launch writes).
+template <class T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+  return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
 template <int D, int FMT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_rows_kernel(AttendArgs a) {
-  using W = WaveRows<D, FMT, 32>;
-  const sbsa_cache8& c = a.c;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int split = (int)(blockIdx.x % a.splits);
-  const int64_t tiles = gridDim.x / a.splits;
-  int s, n, q0;
-  int64_t row0;
-  // late tiles see the most keys: they go first
-  if (!tile_of(a, tiles - 1 - blockIdx.x / a.splits, s, row0, n, q0)) return;
-  LaneRow<32> r;
-  r.find(a, s, (int)blockIdx.y, n, q0, wave * 32 + lane % 32, split);
-  const int64_t token = row0 + r.qi;
-  const bf16_t* qrow = r.there ? a.q + token * a.q_st + r.head * a.q_sh : nullptr;
-  u32x4_t q[D / W::SEG][2];
-#pragma unroll
-  for (int j = 0; j < D / W::SEG; ++j)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) q[j][x] = W::query_piece(qrow, j, x, lane);
-  W w;
-  w.start();
-  const int64_t heads = (int64_t)c.num_seqs * c.num_kv_heads;
-  const int hi = min(r.hi, (r.vis_most + KB - 1) / KB);
-  for (int b = r.lo; b < hi; ++b) {
-    const int64_t place = place_of(c, r.sh, b);
-    typename W::kcodes_t kc;
-    typename W::vcodes_t vc;
-    W::load_k((const uint8_t*)c.codes_k + place * (KB * D), lane, kc);
-    W::load_v((const uint8_t*)c.codes_v + place * (KB * D), lane, vc);
-    typename W::acc_t sc[W::GROUPS];
-    W::scores(kc, [&](int j, int x) { return q[j][x]; }, c.scales[place] * a.scale_log2, sc);
-    u32x4_t p[W::MINE / 8];
-    w.softmax(sc, c.scales[heads * c.num_blocks + place], r.vis - b * KB, (b + 1) * KB <= r.vis_least, lane, p);
-    w.values(vc, p, r.held - b * KB, lane);
+struct RowsTile {
+  static constexpr int BYTES = KB * D;                 // of a block's keys, or values
+  static constexpr int CH = D / 16;                    // pieces of a key row
+  static constexpr int PER_WAVE = BYTES / 1024 / 4;    // loads of 64 pieces by each wave
+  static __device__ __forceinline__ int key_swizzle(int r) {
+    const int x = (r & 3) | ((r >> 5) & 1) << 2;
+    return D == 256 ? x | ((r >> 2) & 1) << 3 : x;
   }
-  w.total();
+  // Load i of a wave takes pieces (4 i + wave) 64 + lane: rows (4 i + wave) 1024 / D + .., whose swizzle depends on
+  // i in the row's bit 5 alone.
+  static __device__ __forceinline__ void load(const uint8_t* kb, const uint8_t* vb, unsigned char* to, int wave, int lane) {
+    const int p = wave * 64 + lane;
+    const int koff = p / CH * D + ((p % CH) ^ key_swizzle(p / CH)) * 16;
+    const int voff = p / 4 * KB + ((p % 4) ^ ((p >> 3) & 3)) * 16;
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)(to + wave * 1024));
+    const u32x4_t krs = codes_rsrc(kb), vrs = codes_rsrc(vb);
+#pragma unroll
+    for (int i = 0; i < PER_WAVE; ++i)
+      lds_load16(krs, at + i * 4096, (uint32_t)((koff ^ (key_swizzle(i * 256 / CH) * 16)) + i * 4096));
+#pragma unroll
+    for (int i = 0; i < PER_WAVE; ++i) lds_load16(vrs, at + BYTES + i * 4096, (uint32_t)(voff + i * 4096));
+  }
+  static __device__ __forceinline__ u32x4_t codes_rsrc(const uint8_t* p) {
+    const uint64_t b = (uint64_t)p;
+    u32x4_t r;                                         // raw buffer resource: base, stride 0, bytes, config
+    r.x = __builtin_amdgcn_readfirstlane((uint32_t)b);
+    r.y = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) & 0xffffu;
+    r.z = (uint32_t)BYTES;
+    r.w = (uint32_t)BUFFER_CONFIG;
+    return r;
+  }
+};
+
+template <int D, int FMT>
+__global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
+  using T = RowsTile<D, FMT>;
+  constexpr int NT = D / 32, STEPS = D / 32;
+  constexpr float P_LOG2 = 11.f, SLACK = 4.f;          // as in WaveRows
+  __shared__ __attribute__((aligned(16))) unsigned char tile[2][2 * T::BYTES];
+  const sbsa_cache8& c = a.c;
+  const int lane = threadIdx.x & 63, part = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  // late tiles see the most keys: they go first
+  const int h = blockIdx.y, slot = (int)(gridDim.x - 1 - blockIdx.x);
+  Share sh;
+  if (!share_of(a, h, slot, sh)) return;
+  LaneRow<32> r;
+  r.find(a, h, sh, wave * 32 + lane % 32);
+  const bf16_t* qrow = r.there ? a.q + r.token * a.q_st + r.head * a.q_sh : nullptr;
+  // the queries in registers, but for what does not fit: that lies in LDS, by wave and lane
+  constexpr int KEPT = D == 256 ? STEPS - 2 : STEPS;
+  __shared__ u32x4_t sq[KEPT < STEPS ? (STEPS - KEPT) * 2 * 256 : 1];
+  bf16x8_t q[KEPT][2];
+#pragma unroll
+  for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const u32x4_t w = WaveRows<D, FMT, 32>::query_piece(qrow, j, x, lane);
+      if (j < KEPT)
+        q[j][x] = as_bf16x8(w);
+      else
+        sq[(2 * (j - KEPT) + x) * 256 + threadIdx.x] = w;
+    }
+  f32x16_t o[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+  float m = -INFINITY, l = 0.f, v_ref = 0.f;
+
+  const int64_t heads = (int64_t)c.num_seqs * c.num_kv_heads;
+  const int64_t head_row = (int64_t)sh.s * c.num_kv_heads + h;
+  const float* scales_v = c.scales + heads * c.num_blocks;
+  auto load = [&](int b, int64_t place) {
+    T::load((const uint8_t*)c.codes_k + place * T::BYTES, (const uint8_t*)c.codes_v + place * T::BYTES, tile[b & 1], wave, lane);
+  };
+  // per-lane places in the tiles: the keys' row of each half (its swizzle does not depend on the half: bits 0, 1, 2
+  // and 5 of the row), the values' row of a 32-dim tile
+  using W = WaveRows<D, FMT, 32>;
+  const int krow = W::key_of(lane % 32, 0);
+  const uint32_t klane = krow * D + ((part ^ T::key_swizzle(krow)) * 16);
+  const uint32_t vlane = (lane % 32) * KB + (((2 * part) ^ ((lane >> 1) & 3)) * 16);
+
+  auto place_at = [&](int b) {                         // as place_of
+    int t = scalar_load(c.table + head_row * c.num_blocks + (b < sh.hi ? b : sh.hi - 1));
+    t = t < 0 ? 0 : t;
+    return head_row * c.num_blocks + (t < c.num_blocks ? t : c.num_blocks - 1);
+  };
+  // places and scales are fetched a block ahead, so that no load is waited for but the tiles'
+  int64_t next_place = 0;
+  float next_ks = 0.f, next_vs = 0.f;
+  if (sh.lo < sh.hi) {
+    const int64_t place = place_at(sh.lo);
+    next_ks = scalar_load(c.scales + place);
+    next_vs = scalar_load(scales_v + place);
+    next_place = place_at(sh.lo + 1);
+    load(sh.lo, place);
+  }
+  for (int b = sh.lo; b < sh.hi; ++b) {
+    const float ks = uniform(next_ks * a.scale_log2), vs = next_vs;
+    const int64_t place = next_place;
+    next_ks = scalar_load(c.scales + place);
+    next_vs = scalar_load(scales_v + place);
+    next_place = place_at(b + 2);
+    // this block's tiles are there, and every wave is done with the last block's
+    __builtin_amdgcn_s_waitcnt(0x0f70);               // vmcnt(0)
+    __syncthreads();
+    if (b + 1 < sh.hi) load(b + 1, place);
+    if (b * KB >= r.vis_most) continue;
+    // a step's or half's piece is a flip of address bits away; laundered, or the compiler keeps every address
+    uint32_t kat = (b & 1) * (2 * T::BYTES) + klane, vat = (b & 1) * (2 * T::BYTES) + T::BYTES + vlane;
+    asm volatile("" : "+v"(kat));
+    asm volatile("" : "+v"(vat));
+    const bool all = (b + 1) * KB <= r.vis_least, whole = sh.held - b * KB >= KB;
+    const int seen = r.vis - b * KB;
+    if (fabsf(vs) > v_ref) {
+      const float f = v_ref / fabsf(vs);
+      v_ref = uniform(fabsf(vs));
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] *= f;
+    }
+    // in (0, 1], or NaN; below 2^-60 fp16 has nothing left of the block's values, but its keys still count
+    float ratio = v_ref > 0.f ? vs / v_ref : vs - vs + 1.f;
+    ratio = ratio < 0x1p-60f ? 0x1p-60f : ratio;
+    const float lift = uniform(P_LOG2 + __builtin_amdgcn_logf(ratio)), drop = uniform(1.f / (ratio * 2048.f));
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      f32x16_t sc;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+      auto query = [&](int j, int x) {
+        return j < KEPT ? q[j < KEPT ? j : 0][x] : as_bf16x8(sq[(2 * (j - KEPT) + x) * 256 + threadIdx.x]);
+      };
+      // a fragment one step ahead; further, and the compiler runs out of registers
+      auto key_piece = [&](int j) {
+        return *reinterpret_cast<const u32x4_t*>(&tile[0][0] + (kat ^ (32u * j)) + 16 * g * D);
+      };
+      u32x4_t ahead = key_piece(0);
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        const u32x4_t w = ahead;
+        if (j + 1 < STEPS) ahead = key_piece(j + 1);
+        sc = W::mfma(decode8<FMT>(w.x, w.y), query(j, 0), sc);
+        sc = W::mfma(decode8<FMT>(w.z, w.w), query(j, 1), sc);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sc[i] *= ks;
+        if (!all && part * 32 + g * 16 + i >= seen) sc[i] = -INFINITY;
+        top = fmaxf(top, sc[i]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      if (__ballot(top > m + SLACK)) {
+        if (__ballot(top == INFINITY)) {               // as in WaveRows
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] = sc[i] == INFINITY ? FLT_MOST : sc[i];
+          top = top == INFINITY ? FLT_MOST : top;
+        }
+        const float to = fmaxf(m, top);
+        const float f = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[t][i] *= f;
+      }
+      // p times the values' relative scale and 2^11, by the exponent; the sum without them
+      const float ref = (m == -INFINITY ? 0.f : m) - lift;
+      u32x4_t p[2];
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        float p0 = __builtin_amdgcn_exp2f(sc[i] - ref), p1 = __builtin_amdgcn_exp2f(sc[i + 1] - ref);
+        if (!all) {                                    // 0 whatever the scale
+          p0 = part * 32 + g * 16 + i >= seen ? 0.f : p0;
+          p1 = part * 32 + g * 16 + i + 1 >= seen ? 0.f : p1;
+        }
+        sum += p0 + p1;
+        p[i / 8][i / 2 % 4] = pack2h(p0, p1);
+      }
+      l += sum * drop;
+      auto value_piece = [&](int t) {
+        return *reinterpret_cast<const u32x4_t*>(&tile[0][0] + (vat ^ (16u * g)) + t * 32 * KB);
+      };
+      ahead = value_piece(0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        u32x4_t w = ahead;
+        if (t + 1 < NT) ahead = value_piece(t + 1);
+        if (!whole) w = clear_past(w, sh.held - b * KB - (part * 32 + g * 16));
+        o[t] = W::mfma(decode8h<FMT>(w.x, w.y), as_f16x8(p[0]), o[t]);
+        o[t] = W::mfma(decode8h<FMT>(w.z, w.w), as_f16x8(p[1]), o[t]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
   if (!r.there) return;
+  const float f = l == 0.f ? 0.f : 0x1p-11f / l;
 #pragma unroll
-  for (int t = 0; t < W::NT; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int x = 0; x < W::NI / 4; ++x) {
+    for (int x = 0; x < 4; ++x) {
       f32x4_t v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = w.o[t][4 * x + i];
-      W::store(a, split, token, r.head, t, x, lane, v);
+      for (int i = 0; i < 4; ++i) v[i] = o[t][4 * x + i] * f * v_ref;
+      r.store(a, h, slot, sh, D, W::dim_of(t, x, lane), v);
     }
-  if (lane < 32) W::store_sum(a, split, token, r.head, w.m, w.l);
+  if (lane < 32) r.store_sum(a, h, slot, sh, m, l);
 }
 
-// The shares of a row joined: a grid block takes 64 dims of a row, 16 threads to a share's 64 dims and every
-// 16th share to each.
+// The shares joined.  The first blocks of the grid each take 64 dims of a row, 16 threads to a share's 64 dims and every
+// 16th share to each; with part_w the others take 256 blocks of keys of a (sequence, head) and
+// add up what the rows left for each of them.
 template <int D>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
-  const int64_t row = blockIdx.x, rows = a.tokens * a.hq;
-  const int lane = threadIdx.x & 63;
-  const int64_t token = row / a.hq;
-  const int head = (int)(row % a.hq);
-  if (a.offsets && (token < a.offsets[0] || token >= a.offsets[a.c.num_seqs])) return;
-  __shared__ f32x4_t fold[16 * 16];
-  const f32x2_t* ml = a.part_ml + row;
-  float top = -INFINITY;
-  for (int x = lane; x < a.splits; x += 64) top = fmaxf(top, ml[x * rows].x);
-  top = wave_max(top);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float total = 0.f;
-  for (int x = lane; x < a.splits; x += 64) {
-    const f32x2_t v = ml[x * rows];
-    total += v.y * __builtin_amdgcn_exp2f(v.x - ref);
-  }
-  total = wave_sum(total);
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  const int d = (int)blockIdx.y * 64 + (threadIdx.x & 15) * 4;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int x = threadIdx.x >> 4; x < a.splits; x += 16) {
-    const f32x2_t v = ml[x * rows];
-    const f32x4_t o = *reinterpret_cast<const f32x4_t*>(a.part_o + (x * rows + row) * D + d);
-    acc += o * (v.y * __builtin_amdgcn_exp2f(v.x - ref) * inv);      // a share without keys has an O of 0
-  }
-  fold[threadIdx.x] = acc;
-  __syncthreads();
-  if (threadIdx.x >= 16) return;
-  f32x4_t sum = fold[threadIdx.x];
-  for (int x = 1; x < 16; ++x) sum += fold[x * 16 + threadIdx.x];
-  u32x2_t w;
-  w.x = pack2bf(sum.x, sum.y);
-  w.y = pack2bf(sum.z, sum.w);
-  *reinterpret_cast<u32x2_t*>(a.out + token * a.o_st + head * a.o_sh + d) = w;
-  if (threadIdx.x == 0 && blockIdx.y == 0) finish_row(a, row, top, total);
-}
-
-// The blocks' weights from the shares that few rows left block by block: a thread per block.
-__global__ __launch_bounds__(256) void weigh_shares_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks) {
+  const int tid = threadIdx.x, lane = tid & 63;
   const sbsa_cache8& c = a.c;
-  const int b = (int)(blockIdx.x * 256 + threadIdx.x), h = blockIdx.y, s = blockIdx.z;
+  if ((int)blockIdx.x < join_blocks) {
+    const int64_t row = blockIdx.x / (D / 64);
+    const int dims = (int)(blockIdx.x % (D / 64)) * 64;
+    const int64_t token = row / a.hq;
+    const int head = (int)(row % a.hq);
+    if (a.offsets && (token < a.offsets[0] || token >= a.offsets[c.num_seqs])) return;
+    const i32x4_t where = a.where[row];
+    if (where.y == 1) return;                          // its one share wrote the result
+    __shared__ f32x4_t fold[16 * 16];
+    const int64_t at = ((int64_t)(head / a.g) * a.slots + where.x) * a.tile_rows + where.z;
+    const f32x2_t* ml = a.part_ml + at;
+    float top = -INFINITY;
+    for (int x = lane; x < where.y; x += 64) top = fmaxf(top, ml[(int64_t)x * a.tile_rows].x);
+    top = wave_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float total = 0.f;
+    for (int x = lane; x < where.y; x += 64) {
+      const f32x2_t v = ml[(int64_t)x * a.tile_rows];
+      total += v.y * __builtin_amdgcn_exp2f(v.x - ref);
+    }
+    total = wave_sum(total);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const int d = dims + (tid & 15) * 4;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int x = tid >> 4; x < where.y; x += 16) {
+      const f32x2_t v = ml[(int64_t)x * a.tile_rows];
+      const f32x4_t o = *reinterpret_cast<const f32x4_t*>(a.part_o + (at + (int64_t)x * a.tile_rows) * D + d);
+      acc += o * (v.y * __builtin_amdgcn_exp2f(v.x - ref) * inv);      // a share without keys has an O of 0
+    }
+    fold[tid] = acc;
+    __syncthreads();
+    if (tid >= 16) return;
+    f32x4_t sum = fold[tid];
+    for (int x = 1; x < 16; ++x) sum += fold[x * 16 + tid];
+    u32x2_t w;
+    w.x = pack2bf(sum.x, sum.y);
+    w.y = pack2bf(sum.z, sum.w);
+    *reinterpret_cast<u32x2_t*>(a.out + token * a.o_st + head * a.o_sh + d) = w;
+    if (tid == 0 && dims == 0) finish_row(a, row, top, total);
+    return;
+  }
+  // the blocks' weights: the rows' sums first (8 threads to a row, 32 rows at a time), then a thread per block
+  const int per_head = (c.num_blocks + 255) / 256;
+  const int i = (int)blockIdx.x - join_blocks, h = i / per_head % c.num_kv_heads, s = i / per_head / c.num_kv_heads;
+  const int b = i % per_head * 256 + tid;
   const int64_t sh = (int64_t)s * c.num_kv_heads + h;
   int64_t row0;
   int n;
   rows_of(a.offsets, s, a.uniform, a.tokens, row0, n);
   const int held = held_of(c, sh);
-  if (n == 0 || b * KB >= held) return;
+  if (i % per_head * 256 * KB >= held) return;         // the same for the whole block
+  __shared__ f32x2_t row_ml[32];
   float sum = 0.f;
-  int qi = b * KB - (held - n);                      // the first row that sees the block
-  for (qi = qi < 0 ? 0 : qi; qi < n; ++qi)
-    for (int j = 0; j < a.g; ++j) {
-      const int64_t row = (row0 + qi) * a.hq + h * a.g + j;
-      const f32x2_t w = a.part_w[row * c.num_blocks + b], all = a.row_ml[row];
+  for (int64_t r0 = 0; r0 < (int64_t)n * a.g; r0 += 32) {
+    const int64_t r = r0 + (tid >> 3);
+    float top = -INFINITY, total = 0.f;
+    i32x4_t where = {0, 0, 0, 0};                      // no shares, past the last row
+    if (r < (int64_t)n * a.g) where = a.where[(row0 + r / a.g) * a.hq + h * a.g + r % a.g];
+    const f32x2_t* ml = a.part_ml + ((int64_t)h * a.slots + where.x) * a.tile_rows + where.z;
+    for (int x = tid & 7; x < where.y; x += 8) top = fmaxf(top, ml[(int64_t)x * a.tile_rows].x);
+#pragma unroll
+    for (int y = 1; y < 8; y <<= 1) top = fmaxf(top, __shfl_xor(top, y, 64));
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int x = tid & 7; x < where.y; x += 8) {
+      const f32x2_t v = ml[(int64_t)x * a.tile_rows];
+      total += v.y * __builtin_amdgcn_exp2f(v.x - ref);
+    }
+#pragma unroll
+    for (int y = 1; y < 8; y <<= 1) total += __shfl_xor(total, y, 64);
+    __syncthreads();
+    if ((tid & 7) == 0) row_ml[tid >> 3] = f32x2_t{top, total == 0.f ? 0.f : 1.f / total};
+    __syncthreads();
+    for (int x = 0; x < 32 && r0 + x < (int64_t)n * a.g; ++x) {
+      const int qi = (int)((r0 + x) / a.g);
+      if (b * KB >= held - n + qi + 1 || b >= c.num_blocks) continue;      // the row does not see the block
+      const f32x2_t w = a.part_w[((row0 + qi) * a.hq + h * a.g + (r0 + x) % a.g) * c.num_blocks + b], all = row_ml[x];
       sum += w.y == 0.f ? 0.f : w.y * __builtin_amdgcn_exp2f(w.x - all.x) * all.y;
     }
-  c.weights[sh * c.num_blocks + b] += sum;
+  }
+  if (n > 0 && b < c.num_blocks && b * KB < held) c.weights[sh * c.num_blocks + b] += sum;
 }
 
 // The attention that each block receives: a wave holds a block of keys and goes over the rows that
@@ -983,9 +1238,10 @@ __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
       hist[tid + EVICT_THREADS] = 0;
       __syncthreads();
       for (int i = mid0 + tid; i < mid1; i += EVICT_THREADS) {
-        const uint32_t k = key(i);
-        if (round == 0 || k >> (SHIFT[round] + WIDTH[round]) == bound >> (SHIFT[round] + WIDTH[round]))
-          atomicAdd(&hist[(k >> SHIFT[round]) & ((1u << WIDTH[round]) - 1)], 1);
+        const uint32_t k = key(i), digit = (k >> SHIFT[round]) & ((1u << WIDTH[round]) - 1);
+        // (digit 0 need not be counted: it is where the bound lies if it is in no other bin)
+        if (digit && (round == 0 || k >> (SHIFT[round] + WIDTH[round]) == bound >> (SHIFT[round] + WIDTH[round])))
+          atomicAdd(&hist[digit], 1);
       }
       __syncthreads();
       // keys in bins above this thread's pair, from the top: threads in reverse order
@@ -999,7 +1255,7 @@ __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
       if (before < wanted && before + h1 >= wanted) {
         s_bin[0] = hi;
         s_bin[1] = before;
-      } else if (before + h1 < wanted && before + h1 + h0 >= wanted) {
+      } else if (before + h1 < wanted && (before + h1 + h0 >= wanted || tid == EVICT_THREADS - 1)) {
         s_bin[0] = hi - 1;
         s_bin[1] = before + h1;
       }
@@ -1090,43 +1346,45 @@ void launch_append(const AppendArgs& a, dim3 grid, hipStream_t stream) {
 // How a call's rows go over the grid.
 struct AttendPlan {
   bool keys;                 // the waves of a block share its rows and split its keys
-  int rows;                  // of a wave
-  int tile_queries, tiles_per_seq, splits;
-  int64_t tiles;
+  int tile_rows, tile_queries;
+  int target;                // shares per KV head to aim for; 0: whole tiles
+  int64_t slots;             // grid blocks per KV head
 };
 
 AttendPlan plan_attend(const sbsa_cache8* c, int num_q_heads, int64_t tokens, int64_t max_rows, bool ragged) {
   AttendPlan p;
   const int g = num_q_heads / c->num_kv_heads;
   const int64_t uniform = tokens / c->num_seqs;
-  int64_t most = ragged ? (max_rows < 1 || max_rows > tokens ? tokens : max_rows) : uniform;
+  const int64_t most = ragged ? (max_rows < 1 || max_rows > tokens ? tokens : max_rows) : uniform;
   p.keys = most * g <= 32;
-  p.rows = most * g <= 16 ? 16 : 32;
-  p.tile_queries = (p.keys ? p.rows : 4 * p.rows) / g;
-  p.tiles_per_seq = (int)((uniform + p.tile_queries - 1) / p.tile_queries);
-  p.tiles = ragged ? tokens / p.tile_queries + c->num_seqs : (int64_t)p.tiles_per_seq * c->num_seqs;
-  // enough grid blocks for two per compute unit of the card's 256, each with a block of keys per wave at least
-  const int64_t have = p.tiles * c->num_kv_heads;
-  int64_t splits = 512 / (have > 0 ? have : 1);
-  const int64_t most_splits = (c->num_blocks + 3) / 4;
-  splits = splits < most_splits ? splits : most_splits;
-  p.splits = splits < 1 ? 1 : (int)splits;
+  p.tile_rows = !p.keys ? 128 : most * g <= 16 ? 16 : 32;
+  p.tile_queries = p.tile_rows / g;
+  const int64_t tiles = ragged ? tokens / p.tile_queries + c->num_seqs
+                               : (uniform + p.tile_queries - 1) / p.tile_queries * c->num_seqs;
+  // The keys are shared out until there are two grid blocks for each of the card's 256 compute units; a
+  // tile of few rows or of few keys stays whole, which saves the join.
+  const int64_t heads = c->num_kv_heads;
+  p.target = 0;
+  if (tiles * heads < 512 && c->num_blocks > 16) p.target = (int)(512 / heads < 1 ? 1 : 512 / heads);
+  p.slots = tiles + p.target;
   return p;
 }
 
-// The workspace's parts, in floats: the shares' O and sums, the rows' sums, and each row's sums block by block.
+// The workspace's parts, in floats: the shares' O and sums, where each row's shares lie, the rows' sums, and each
+// row's sums block by block.
 struct AttendSpace {
-  size_t o, part, row, w;
-  size_t bytes() const { return (o + part + row + w) * sizeof(float); }
+  size_t o, part, where, row, w;
+  size_t bytes() const { return (o + part + where + row + w) * sizeof(float); }
 };
 
 AttendSpace attend_space(const AttendPlan& p, const sbsa_cache8* c, int64_t tokens, int num_q_heads, bool accumulate) {
-  const size_t rows = (size_t)tokens * num_q_heads;
+  const size_t rows = (size_t)tokens * num_q_heads, shares = p.target ? (size_t)c->num_kv_heads * p.slots * p.tile_rows : 0;
   AttendSpace x;
-  x.o = p.splits > 1 ? p.splits * rows * c->head_dim : 0;
-  x.part = p.splits > 1 ? 2 * p.splits * rows : 0;
-  x.row = accumulate ? 2 * rows : 0;
-  x.w = accumulate && p.keys ? 2 * rows * c->num_blocks : 0;
+  x.o = shares * c->head_dim;
+  x.part = 2 * shares;
+  x.where = p.target ? 4 * rows : 0;
+  x.row = accumulate && !(p.keys && p.target) ? (2 * rows + 3) / 4 * 4 : 0;
+  x.w = accumulate && p.keys && p.target ? 2 * rows * c->num_blocks : 0;
   return x;
 }
 
@@ -1142,18 +1400,17 @@ bool launch_keys(const AttendArgs& a, dim3 grid, hipStream_t stream) {
 
 template <int D, int FMT>
 bool launch_attend(const AttendArgs& a, const AttendPlan& p, int accumulate, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.tiles * p.splits), (unsigned)a.c.num_kv_heads);
-  if (p.keys) {
-    if (!(p.rows == 16 ? launch_keys<D, FMT, 16>(a, grid, stream) : launch_keys<D, FMT, 32>(a, grid, stream))) return false;
-  } else {
+  const dim3 grid((unsigned)p.slots, (unsigned)a.c.num_kv_heads);
+  if (!p.keys)
     hipLaunchKernelGGL((attend_rows_kernel<D, FMT>), grid, dim3(256), 0, stream, a);
+  else if (!(p.tile_rows == 16 ? launch_keys<D, FMT, 16>(a, grid, stream) : launch_keys<D, FMT, 32>(a, grid, stream)))
+    return false;
+  if (p.target) {
+    const int64_t join = a.tokens * a.hq * (D / 64);
+    const int64_t weigh = a.part_w ? (int64_t)((a.c.num_blocks + 255) / 256) * a.c.num_kv_heads * a.c.num_seqs : 0;
+    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(join + weigh)), dim3(256), 0, stream, a, (int)join);
   }
-  if (p.splits > 1)
-    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.tokens * a.hq), D / 64), dim3(256), 0, stream, a);
-  if (accumulate && p.keys)
-    hipLaunchKernelGGL(weigh_shares_kernel, dim3((unsigned)((a.c.num_blocks + 255) / 256), (unsigned)a.c.num_kv_heads,
-                                                 (unsigned)a.c.num_seqs), dim3(256), 0, stream, a);
-  else if (accumulate)
+  if (accumulate && !a.part_w)
     hipLaunchKernelGGL((weigh_kernel<D, FMT>),
                        dim3((unsigned)((a.c.num_blocks + 3) / 4), (unsigned)a.c.num_kv_heads, (unsigned)a.c.num_seqs),
                        dim3(256), 0, stream, a);
@@ -1210,7 +1467,9 @@ extern "C" int sbsa_cache8_attend(const sbsa_cache8* cache, const void* q, int64
     return SBSA_ERR_UNSUPPORTED;
   if (tokens == 0) return SBSA_OK;
   const AttendPlan p = plan_attend(cache, num_q_heads, tokens, max_rows, offsets != nullptr);
-  if (p.tiles * p.splits >= (1 << 24)) return SBSA_ERR_UNSUPPORTED;
+  if (p.slots >= (1 << 24) ||
+      (int64_t)cache->num_blocks * cache->num_kv_heads * cache->num_seqs / 256 + tokens * num_q_heads * 4 >= (1 << 24))
+    return SBSA_ERR_UNSUPPORTED;
   const AttendSpace space = attend_space(p, cache, tokens, num_q_heads, accumulate != 0);
   if (workspace_bytes < space.bytes()) return SBSA_ERR_CAPACITY;
   if (space.bytes() > 0 && (!workspace || (uintptr_t)workspace % 16)) return SBSA_ERR_ARG;
@@ -1219,12 +1478,17 @@ extern "C" int sbsa_cache8_attend(const sbsa_cache8* cache, const void* q, int64
   a.q = (const bf16_t*)q; a.q_st = q_st; a.q_sh = q_sh;
   a.out = (bf16_t*)out; a.o_st = o_st; a.o_sh = o_sh; a.lse = lse;
   a.part_o = (float*)workspace;
-  a.part_ml = (f32x2_t*)(a.part_o + space.o);
-  a.row_ml = accumulate ? (f32x2_t*)(a.part_o + space.o + space.part) : nullptr;
-  a.part_w = space.w ? (f32x2_t*)(a.part_o + space.o + space.part + space.row) : nullptr;
+  float* at = a.part_o + space.o;
+  a.part_ml = (f32x2_t*)at;
+  at += space.part;
+  a.where = (i32x4_t*)at;
+  at += space.where;
+  a.row_ml = space.row ? (f32x2_t*)at : nullptr;
+  at += space.row;
+  a.part_w = space.w ? (f32x2_t*)at : nullptr;
   a.offsets = offsets; a.tokens = tokens; a.uniform = tokens / cache->num_seqs;
   a.hq = num_q_heads; a.g = num_q_heads / cache->num_kv_heads;
-  a.splits = p.splits; a.tile_queries = p.tile_queries; a.tiles_per_seq = p.tiles_per_seq;
+  a.tile_queries = p.tile_queries; a.tile_rows = p.tile_rows; a.slots = (int)p.slots; a.target = p.target;
   a.scale_log2 = sm_scale * LOG2E;
   const bool e4m3 = cache->format == SBSA_CACHE8_E4M3;
   const bool ok = cache->head_dim == 128

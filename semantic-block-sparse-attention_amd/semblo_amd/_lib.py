@@ -129,8 +129,14 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+# The handle itself, without the Stream object around it (a tenth of the time), where torch has the call
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream(device: torch.device | None = None) -> int:
     """The current torch stream's hipStream_t."""
+    if _RAW_STREAM is not None and device is not None and device.index is not None:
+        return _RAW_STREAM(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -143,10 +149,10 @@ def require_device(*tensors: torch.Tensor) -> None:
 def require_one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
     """Every tensor of a call lies on one ROCm device."""
     require_device(first)
-    device = first.device
+    device = first.get_device()
     for t in others:
-        if t is not None and t.device != device:
-            raise RuntimeError(f"one call's tensors lie on {device} and {t.device}")
+        if t is not None and t.get_device() != device:
+            raise RuntimeError(f"one call's tensors lie on {first.device} and {t.device}")
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -164,6 +170,9 @@ def call_on(device: torch.device, name: str, *args) -> int:
     """``call`` with the device's current torch stream as the last argument, the device made current
     for the launch where it is not."""
     if device.type != "cuda" or device.index == torch.cuda.current_device():
-        return call(name, *args, stream(device))
+        rc = getattr(_LIB or load(), name)(*args, stream(device))
+        if rc != 0:
+            raise RuntimeError(f"{name} failed: {ERRORS.get(rc, rc)}")
+        return rc
     with torch.cuda.device(device):
         return call(name, *args, stream(device))

@@ -101,9 +101,9 @@ class CacheTables:
         s, h, n = self.table.shape
         _lib.require_one_device(self.table, self.weights, self.lengths, self.open_block, out.table, out.weights,
                                 out.lengths, out.open_block)
-        _lib.call_on(self.table.device, "sbsa_cache8_evict", _lib.ptr(self.table), _lib.ptr(self.weights),
-                     _lib.ptr(self.lengths), _lib.ptr(self.open_block), _lib.ptr(out.table), _lib.ptr(out.weights),
-                     _lib.ptr(out.lengths), _lib.ptr(out.open_block), s, h, n, keep, sink, recent)
+        _lib.call_on(self.table.device, "sbsa_cache8_evict", self.table.data_ptr(), self.weights.data_ptr(),
+                     self.lengths.data_ptr(), self.open_block.data_ptr(), out.table.data_ptr(), out.weights.data_ptr(),
+                     out.lengths.data_ptr(), out.open_block.data_ptr(), s, h, n, keep, sink, recent)
         return out
 
 
@@ -154,6 +154,8 @@ class QuantizedKVCache:
                                     tables.open_block, self._counters, self._counters[s * h:])),
             s, h, n, d, FORMATS[fmt])
         self._ref = ctypes.byref(self._struct)
+        self._scale = d ** -0.5
+        self._needs: dict = {}          # workspace bytes by a call's sizes
 
     @property
     def capacity(self) -> int:
@@ -184,9 +186,10 @@ class QuantizedKVCache:
             self._counters.zero_()
 
     def _rows(self, x: torch.Tensor, what: str, heads: int | None) -> torch.Tensor:
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             raise ValueError(f"{what} must be [tokens, {heads or 'heads'}, {self.head_dim}], got {list(x.shape)}")
-        if x.dtype != torch.bfloat16:
+        if x.dtype is not torch.bfloat16:
             raise ValueError(f"{what} must be bfloat16, got {x.dtype}")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("the 8-bit cache has no backward pass: call it under torch.no_grad()")
@@ -203,7 +206,7 @@ class QuantizedKVCache:
                 raise ValueError(f"{tokens} rows do not go evenly over {self.num_seqs} sequences: pass offsets")
             return None, 0
         _check(offsets, "offsets", (self.num_seqs + 1,), torch.int32)
-        return _lib.ptr(offsets), int(max_rows or 0)
+        return offsets.data_ptr(), int(max_rows or 0)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, *, offsets: torch.Tensor | None = None,
                start: torch.Tensor | None = None, max_rows: int | None = None) -> None:
@@ -225,8 +228,10 @@ class QuantizedKVCache:
         if start is not None:
             _check(start, "start", (self.num_seqs,), torch.int32)
         _lib.require_one_device(self.codes_k, k, v, offsets, start)
-        _lib.call_on(self.device, "sbsa_cache8_append", self._ref, _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(v),
-                     v.stride(0), v.stride(1), tokens, at, _lib.ptr(start), hint)
+        kst, ksh, _ = k.stride()
+        vst, vsh, _ = v.stride()
+        _lib.call_on(self.device, "sbsa_cache8_append", self._ref, k.data_ptr(), kst, ksh, v.data_ptr(), vst, vsh, tokens,
+                     at, None if start is None else start.data_ptr(), hint)
 
     def attend(self, q: torch.Tensor, *, offsets: torch.Tensor | None = None, max_rows: int | None = None,
                sm_scale: float | None = None, accumulate: bool = False, return_lse: bool = False,
@@ -242,6 +247,7 @@ class QuantizedKVCache:
         if hq < 1 or hq % self.num_kv_heads or hq // self.num_kv_heads > 16:
             raise ValueError(f"{hq} query heads on {self.num_kv_heads} KV heads: 1 to 16 of them to each")
         at, hint = self._spread(tokens, offsets, max_rows)
+        accumulate = bool(accumulate)
         if out is None:
             out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(0) % 8 or \
@@ -249,14 +255,23 @@ class QuantizedKVCache:
             raise ValueError(f"out must be bfloat16 {list(q.shape)} with rows on 16 bytes")
         elif _lib.overlap(out, q):
             raise ValueError("out overlaps q")
-        lse = torch.empty((tokens, hq), dtype=torch.float32, device=q.device) if return_lse else None
         _lib.require_one_device(self.codes_k, q, out, offsets)
-        need = _lib.query("sbsa_cache8_attend_workspace_bytes", self._ref, hq, tokens, hint, int(at is not None),
-                          int(accumulate))
-        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _lib.call_on(self.device, "sbsa_cache8_attend", self._ref, _lib.ptr(q), q.stride(0), q.stride(1), hq, tokens, at,
-                     hint, self.head_dim ** -0.5 if sm_scale is None else float(sm_scale), _lib.ptr(out), out.stride(0),
-                     out.stride(1), _lib.ptr(lse), int(accumulate), _lib.ptr(work), need)
+        lse = torch.empty((tokens, hq), dtype=torch.float32, device=self.device) if return_lse else None
+        # the workspace goes by sizes that the host knows; made anew by each call, so that captured graphs and streams have
+        # their own
+        key = (hq, tokens, hint, at is None, accumulate)
+        need = self._needs.get(key)
+        if need is None:
+            if len(self._needs) > 4096:
+                self._needs.clear()
+            need = self._needs[key] = _lib.query("sbsa_cache8_attend_workspace_bytes", self._ref, hq, tokens, hint,
+                                                 at is not None, accumulate)
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        qst, qsh, _ = q.stride()
+        ost, osh, _ = out.stride()
+        _lib.call_on(self.device, "sbsa_cache8_attend", self._ref, q.data_ptr(), qst, qsh, hq, tokens, at, hint,
+                     self._scale if sm_scale is None else sm_scale, out.data_ptr(), ost, osh,
+                     None if lse is None else lse.data_ptr(), accumulate, None if work is None else work.data_ptr(), need)
         return (out, lse) if return_lse else out
 
     def evict(self, keep: int, *, sink: int = 0, recent: int = 1) -> None:

@@ -127,9 +127,10 @@ class RotaryEmbedding:
         return tables
 
     def _rows(self, x: torch.Tensor, what: str, tokens: int) -> None:
-        if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != self.head_dim:
+        shape = x.shape
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != self.head_dim:
             raise ValueError(f"{what} must be [{tokens}, heads, {self.head_dim}], got {list(x.shape)}")
-        if x.dtype != torch.bfloat16 or x.stride(2) != 1:
+        if x.dtype is not torch.bfloat16 or x.stride(2) != 1:
             raise ValueError(f"{what} must be bfloat16 with a unit inner stride")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("the rotary embedding has no backward pass: call it under torch.no_grad()")
@@ -142,31 +143,37 @@ class RotaryEmbedding:
         ``inverse`` rotates back (keys before the embedding from a cache's)."""
         tokens = q.shape[0]
         self._rows(q, "q", tokens)
-        if positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype is not torch.int64 and positions.dtype is not torch.int32:
             raise ValueError("positions must be int32 or int64")
         if positions.shape != ((tokens,) if self._axes is None else (self.num_axes, tokens)):
             raise ValueError(f"positions must be {[tokens] if self._axes is None else [self.num_axes, tokens]}, "
                              f"got {list(positions.shape)}")
+        device = q.device
         if out_q is None:
-            out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out_q = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
         else:
             self._output(out_q, q, "out_q")
-        if k is not None:
+        qst, qsh, _ = q.stride()
+        ost, osh, _ = out_q.stride()
+        if k is None:
+            if out_k is not None:
+                raise ValueError("out_k without k")
+            kv = (None, 0, 0, None, 0, 0, 0)
+        else:
             self._rows(k, "k", tokens)
             if out_k is None:
-                out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+                out_k = torch.empty(k.shape, dtype=torch.bfloat16, device=device)
             else:
                 self._output(out_k, k, "out_k")
-        elif out_k is not None:
-            raise ValueError("out_k without k")
-        turns, axes = self._tables(q.device)
+            kst, ksh, _ = k.stride()
+            okst, oksh, _ = out_k.stride()
+            kv = (k.data_ptr(), kst, ksh, out_k.data_ptr(), okst, oksh, k.shape[1])
         _lib.require_one_device(q, out_q, positions, k, out_k)
-        kv = (_lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(out_k), out_k.stride(0), out_k.stride(1),
-              k.shape[1]) if k is not None else (None, 0, 0, None, 0, 0, 0)
-        _lib.call_on(q.device, "sbsa_rotary", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(out_q), out_q.stride(0),
-                     out_q.stride(1), q.shape[1], *kv, _lib.ptr(positions), positions.element_size(),
-                     positions.stride(0) if axes is not None else 0, positions.stride(-1), tokens, self.head_dim,
-                     self.rotary_dim, int(self.interleaved), _lib.ptr(turns), _lib.ptr(axes), self.gain, int(inverse))
+        turns, axes = self._tables(device)
+        _lib.call_on(device, "sbsa_rotary", q.data_ptr(), qst, qsh, out_q.data_ptr(), ost, osh, q.shape[1], *kv,
+                     positions.data_ptr(), positions.element_size(), positions.stride(0) if axes is not None else 0,
+                     positions.stride(-1), tokens, self.head_dim, self.rotary_dim, self.interleaved, turns.data_ptr(),
+                     None if axes is None else axes.data_ptr(), self.gain, inverse)
         return out_q if k is None else (out_q, out_k)
 
     def _output(self, out: torch.Tensor, x: torch.Tensor, what: str) -> None:
