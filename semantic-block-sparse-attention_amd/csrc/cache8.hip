@@ -105,6 +105,28 @@ __device__ __forceinline__ uint32_t encode2(float x, float y) {
   }
 }
 
+// a value that is the same in every lane, in a scalar register
+__device__ __forceinline__ float uniform(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(v)));
+}
+
+// a value joined with the one 32 (or 16) lanes away, without a round trip through LDS
+__device__ __forceinline__ float max32(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float max16(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+
+// the lane's number, counted anew
+__device__ __forceinline__ int lane_again() {
+  int l = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
 __device__ __forceinline__ int64_t place_of(const sbsa_cache8& c, int64_t sh, int block) {
   int t = c.table[sh * c.num_blocks + block];
   t = t < 0 ? 0 : t;
@@ -154,12 +176,14 @@ __device__ __forceinline__ float quotient(float x, float s, float inv) {
 
 typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 
-// A block of the grid takes a block of 64 tokens (and every gridDim.x-th after it) of one
-// (sequence, head): its rows into registers, the largest magnitudes of the keys and of the values over the block, the
-// codes out.  A thread holds PASSES consecutive rows of 8 columns, so its codes of a key row are 8 bytes of it and
-// those of a value column PASSES bytes of that; the values' turn through LDS only to leave in whole rows of
-// [dim][64].  The last of a (sequence, head)'s grid blocks to end moves the length on, so that none reads a moved one.
-template <int D, int FMT>
+// A block of the grid takes the keys (even grid x) or the values (odd) of a block of 64 tokens of one
+// (sequence, head), and of every gridDim.x / 2-th block after it: its rows into registers, the largest magnitude
+// over the block, the codes out.  A thread holds PASSES consecutive rows of 8 columns, so its codes of a key row are 8
+// bytes of it and those of a value column PASSES bytes of that; the values' turn through LDS only to leave in
+// whole rows of [dim][64].  No grid block moves a length that another may still read:
+// ONE: the call touches one block of a (sequence, head) at most, and the last of its two grid blocks (by a ticket) moves the
+// length on; otherwise append_end_kernel does (tickets of a long prompt's 1000 grid blocks on one address took as long as the rest).
+template <int D, int FMT, bool ONE>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int CH = D / 8;             // 16-byte pieces of a row
   constexpr int PASSES = KB * CH / 256; // consecutive rows of a thread: 4 or 8
@@ -167,11 +191,11 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr float CODE_MAX = FMT == SBSA_CACHE8_E4M3 ? 448.f : 127.f;
   const sbsa_cache8& c = a.c;
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
+  const int t = blockIdx.x & 1, bx = blockIdx.x >> 1, step = gridDim.x >> 1;
   const int64_t sh = (int64_t)s * c.num_kv_heads + h;
   const int64_t heads = (int64_t)c.num_seqs * c.num_kv_heads;
-  __shared__ int red[2][4];
+  __shared__ int red[4];
   __shared__ __attribute__((aligned(16))) unsigned char turn[D * LD];
-  __shared__ int s_last;
 
   int64_t row0;
   int n;
@@ -188,136 +212,157 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int first = start / KB, last = grows ? (end - 1) / KB : first - 1;
 
   const int col = (tid % CH) * 8, r0 = tid / CH * PASSES;
-  const bf16_t* src[2] = {a.k + row0 * a.k_st + h * a.k_sh, a.v + row0 * a.v_st + h * a.v_sh};
-  const int64_t st[2] = {a.k_st, a.v_st};
-  bf16_t* const tail = (bf16_t*)c.tail + sh * KB * D;
-  const int64_t tail_v = heads * KB * D, scale_v = heads * c.num_blocks;
-  for (int b = first + (int)blockIdx.x; b <= last; b += (int)gridDim.x) {
+  const bf16_t* const src = t ? a.v + row0 * a.v_st + h * a.v_sh : a.k + row0 * a.k_st + h * a.k_sh;
+  const int64_t st = t ? a.v_st : a.k_st;
+  bf16_t* const tail = (bf16_t*)c.tail + (t * heads + sh) * KB * D;
+  float* const scales = c.scales + t * heads * c.num_blocks;
+  for (int b = first + bx; b <= last; b += step) {
     const int64_t place = place_of(c, sh, b);
-    uint8_t* const codes[2] = {(uint8_t*)c.codes_k + place * KB * D, (uint8_t*)c.codes_v + place * KB * D};
-    u32x4_t x[2][PASSES];
-    const bool fresh = b * KB >= start && (b + 1) * KB <= end;     // the block is new rows throughout
-    if (fresh) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p)
-          x[t][p] = *reinterpret_cast<const u32x4_t*>(src[t] + (int64_t)(b * KB + r0 + p - start) * st[t] + col);
-    } else {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-          const int j = r0 + p, pos = b * KB + j;
-          u32x4_t w = {0u, 0u, 0u, 0u};
-          if (pos >= start && pos < end) {
-            w = *reinterpret_cast<const u32x4_t*>(src[t] + (int64_t)(pos - start) * st[t] + col);
-          } else if (pos < start && open == b) {
-            w = *reinterpret_cast<const u32x4_t*>(tail + t * tail_v + j * D + col);
-          } else if (pos < start) {
-            // the row is there in its codes alone
-            const float old = c.scales[t * scale_v + place];
-            bf16_t y[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              y[i] = f2bf(decode1<FMT>(codes[t][t ? (col + i) * KB + j : j * D + col + i]) * old);
-            __builtin_memcpy(&w, y, 16);
-          }
-          x[t][p] = w;
-        }
-    }
-    // the largest magnitudes, as bf16 bits without the sign: those that are not finite are 0x7f80 and up
-    float scale[2];
-    bool fine[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      u16x2_t most = {0, 0};
+    uint8_t* const codes = (t ? (uint8_t*)c.codes_v : (uint8_t*)c.codes_k) + place * KB * D;
+    u32x4_t x[PASSES];
+    if (b * KB >= start && (b + 1) * KB <= end) {     // the block is new rows throughout
 #pragma unroll
       for (int p = 0; p < PASSES; ++p)
+        x[p] = *reinterpret_cast<const u32x4_t*>(src + (int64_t)(b * KB + r0 + p - start) * st + col);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w = x[t][p][i] & 0x7fff7fffu;
-          u16x2_t v;
-          __builtin_memcpy(&v, &w, 4);
-          most = __builtin_elementwise_max(most, v);
+      for (int p = 0; p < PASSES; ++p) {
+        const int j = r0 + p, pos = b * KB + j;
+        u32x4_t w = {0u, 0u, 0u, 0u};
+        if (pos >= start && pos < end) {
+          w = *reinterpret_cast<const u32x4_t*>(src + (int64_t)(pos - start) * st + col);
+        } else if (pos < start && open == b) {
+          w = *reinterpret_cast<const u32x4_t*>(tail + j * D + col);
+        } else if (pos < start) {
+          // the row is there in its codes alone
+          const float old = scales[place];
+          const int at = t ? col * KB + j : j * D + col, by = t ? KB : 1;
+          uint64_t half[2] = {0, 0};
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {               // (rolled: rare, and 64 loads' addresses if not)
+            const uint64_t y = f2bf(decode1<FMT>(codes[at + i * by]) * old);
+            half[1] = half[1] >> 16 | half[0] << 48;
+            half[0] = half[0] >> 16 | y << 48;
+          }
+          w.x = (uint32_t)half[1]; w.y = (uint32_t)(half[1] >> 32);
+          w.z = (uint32_t)half[0]; w.w = (uint32_t)(half[0] >> 32);
         }
-      int m = most.x > most.y ? most.x : most.y;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
-      if ((tid & 63) == 0) red[t][tid >> 6] = m;
-    }
-    __syncthreads();                    // and every row is read before a code or the tail is written
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int m = max(max(red[t][0], red[t][1]), max(red[t][2], red[t][3]));
-      fine[t] = m < 0x7f80;
-      scale[t] = fine[t] ? fmaxf(bf2f((bf16_t)m) / CODE_MAX, 0x1p-126f) : __uint_as_float(0x7fc00000u);
-      if (tid == 0) c.scales[t * scale_v + place] = scale[t];
-    }
-    const bool easy = scale[0] >= 0x1p-90f && scale[1] >= 0x1p-90f;      // (no, where one is NaN)
-    const float inv[2] = {1.f / scale[0], 1.f / scale[1]};
-    auto value = [&](int t, int p, int i) {
-      const uint32_t w = x[t][p][i >> 1];
-      const float v = bf2f((bf16_t)(i & 1 ? w >> 16 : w & 0xffffu));
-      return easy ? quotient(v, scale[t], inv[t]) : v / scale[t];
-    };
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      uint32_t w[2] = {0u, 0u};
-      if (fine[0]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i >> 1] |= encode2<FMT>(value(0, p, 2 * i), value(0, p, 2 * i + 1)) << (16 * (i & 1));
+        x[p] = w;
       }
-      u32x2_t o;
-      o.x = w[0]; o.y = w[1];
-      *reinterpret_cast<u32x2_t*>(codes[0] + (r0 + p) * D + col) = o;
     }
+    // the largest magnitude, as bf16 bits without the sign: one that is not finite is 0x7f80 and up
+    u16x2_t top = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t w[PASSES / 4];
+    for (int p = 0; p < PASSES; ++p)
 #pragma unroll
-      for (int x4 = 0; x4 < PASSES / 4; ++x4)
-        w[x4] = fine[1] ? encode2<FMT>(value(1, 4 * x4, i), value(1, 4 * x4 + 1, i)) |
-                              encode2<FMT>(value(1, 4 * x4 + 2, i), value(1, 4 * x4 + 3, i)) << 16
-                        : 0u;
-      __builtin_memcpy(turn + (col + i) * LD + r0, w, PASSES);
-    }
-    if (b == last && first == last) {
-      // the rows are kept: those that were the tail's already are there
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = x[p][i] & 0x7fff7fffu;
+        u16x2_t v;
+        __builtin_memcpy(&v, &w, 4);
+        top = __builtin_elementwise_max(top, v);
+      }
+    int most = top.x > top.y ? top.x : top.y;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = most;
+    __syncthreads();                    // and every row is read before a code or the tail is written
+    most = max(max(red[0], red[1]), max(red[2], red[3]));
+    const bool fine = most < 0x7f80;
+    const float scale = fine ? fmaxf(bf2f((bf16_t)most) / CODE_MAX, 0x1p-126f) : __uint_as_float(0x7fc00000u);
+    if (tid == 0) scales[place] = scale;
+    const bool easy = scale >= 0x1p-90f;              // (no, where it is NaN)
+    const float inv = 1.f / scale;
+    // (a row or column at a time: the compiler would hold every quotient, and twice, for both divisions)
+    auto codes_out = [&](auto&& divide) {
+      auto value = [&](int p, int i) {
+        const uint32_t w = x[p][i >> 1];
+        return divide(bf2f((bf16_t)(i & 1 ? w >> 16 : w & 0xffffu)));
+      };
+      if (t == 0) {
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
-          const int pos = b * KB + r0 + p;
-          if (pos < end && (pos >= start || open != b))
-            *reinterpret_cast<u32x4_t*>(tail + t * tail_v + (r0 + p) * D + col) = x[t][p];
-        }
-    }
-    __syncthreads();
+          u32x2_t o;
 #pragma unroll
-    for (int i = tid; i < D * (KB / 16); i += 256)
-      *reinterpret_cast<u32x4_t*>(codes[1] + i * 16) = *reinterpret_cast<const u32x4_t*>(turn + (i / 4) * LD + (i % 4) * 16);
-    if (b * KB >= start && tid == 0) c.weights[sh * c.num_blocks + b] = 0.f;
-    __syncthreads();                    // LDS is used again
+          for (int i = 0; i < 2; ++i)
+            o[i] = encode2<FMT>(value(p, 4 * i), value(p, 4 * i + 1)) | encode2<FMT>(value(p, 4 * i + 2), value(p, 4 * i + 3)) << 16;
+          *reinterpret_cast<u32x2_t*>(codes + (r0 + p) * D + col) = o;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t w[PASSES / 4];
+#pragma unroll
+          for (int q = 0; q < PASSES / 4; ++q)
+            w[q] = encode2<FMT>(value(4 * q, i), value(4 * q + 1, i)) | encode2<FMT>(value(4 * q + 2, i), value(4 * q + 3, i)) << 16;
+          __builtin_memcpy(turn + (col + i) * LD + r0, w, PASSES);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+    if (easy)
+      codes_out([&](float v) { return quotient(v, scale, inv); });
+    else if (fine)
+      codes_out([&](float v) { return v / scale; });
+    else
+      codes_out([&](float) { return 0.f; });
+    if (b == last && (ONE || first == last)) {
+      // the rows are kept: those that were the tail's already are there (another grid block may still read the tail
+      // otherwise)
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int pos = b * KB + r0 + p;
+        if (pos < end && (pos >= start || open != b)) *reinterpret_cast<u32x4_t*>(tail + (r0 + p) * D + col) = x[p];
+      }
+    }
+    if (t == 0 && b * KB >= start && tid == 0) c.weights[sh * c.num_blocks + b] = 0.f;
+    __syncthreads();
+    if (t == 1) {
+#pragma unroll
+      for (int i = tid; i < D * (KB / 16); i += 256)
+        *reinterpret_cast<u32x4_t*>(codes + i * 16) = *reinterpret_cast<const u32x4_t*>(turn + (i / 4) * LD + (i % 4) * 16);
+      __syncthreads();                  // LDS is used again
+    }
   }
 
-  if (gridDim.x > 1) {
-    // Every read of this block has ended (its values were used before the barrier above, or are by the next), so the
-    // ticket needs no fence: a release would write the XCD's L2 back, 2000 times in a long prompt (133 us to 50).
-    __syncthreads();
-    if (tid == 0) s_last = atomicAdd(&c.counters[sh], 1) == (int)gridDim.x - 1;
-    __syncthreads();
-    if (!s_last) return;
-    if (tid == 0) c.counters[sh] = 0;
-    // the last block's rows are kept: all of them are new where it is not the first
-    for (int t = 0; t < 2 && last > first; ++t)
-      for (int j = r0; j < r0 + PASSES && last * KB + j < end; ++j)
-        *reinterpret_cast<u32x4_t*>(tail + t * tail_v + j * D + col) =
-            *reinterpret_cast<const u32x4_t*>(src[t] + (int64_t)(last * KB + j - start) * st[t] + col);
-  }
-  if (tid == 0) {
+  if constexpr (!ONE) return;
+  // Every read of this block has ended (its values were used before the barriers above), so the ticket needs no fence.
+  __syncthreads();
+  if (tid == 0 && atomicAdd(&c.counters[sh], 1) == 1) {
+    c.counters[sh] = 0;
     c.lengths[sh] = end;
     if (grows) c.open_block[sh] = last;
+  }
+}
+
+// The lengths moved on, and the last block's rows kept: all of them are new where it is not the first.
+template <int D>
+__global__ __launch_bounds__(256) void append_end_kernel(AppendArgs a) {
+  const sbsa_cache8& c = a.c;
+  const int h = blockIdx.x, s = blockIdx.y;
+  const int64_t sh = (int64_t)s * c.num_kv_heads + h, heads = (int64_t)c.num_seqs * c.num_kv_heads;
+  int64_t row0;
+  int n;
+  rows_of(a.offsets, s, a.uniform, a.tokens, row0, n);
+  const int held = held_of(c, sh), room = c.num_blocks * KB;
+  int start = a.start ? a.start[s] : held;
+  start = start < 0 ? 0 : (start < held ? start : held);
+  const int end = (int64_t)start + n > room ? room : start + n;
+  const int first = start / KB, last = end > start ? (end - 1) / KB : -1;
+  __syncthreads();                      // the length is read
+  if (threadIdx.x == 0) {
+    c.lengths[sh] = end;
+    if (last >= 0) c.open_block[sh] = last;
+  }
+  if (last <= first) return;
+  constexpr int CH = D / 8;
+  for (int i = threadIdx.x; i < 2 * KB * CH; i += 256) {
+    const int t = i / (KB * CH), j = i / CH % KB, col = i % CH * 8;
+    if (last * KB + j >= end) continue;
+    const bf16_t* from = t ? a.v + h * a.v_sh + (row0 + last * KB + j - start) * a.v_st
+                           : a.k + h * a.k_sh + (row0 + last * KB + j - start) * a.k_st;
+    *reinterpret_cast<u32x4_t*>((bf16_t*)c.tail + ((t * heads + sh) * KB + j) * D + col) =
+        *reinterpret_cast<const u32x4_t*>(from + col);
   }
 }
 
@@ -375,7 +420,7 @@ __device__ __forceinline__ bool share_of(const AttendArgs& a, int h, int slot, S
       look(s0 + lane, r, m, e, t, b);
       total += t * b;
     }
-    total = wave_sum_i32(total);
+    total = wave_sum_i32_dpp(total);
     per = (total + a.target - 1) / a.target;
     per = per < 4 ? 4 : per;
   }
@@ -383,7 +428,7 @@ __device__ __forceinline__ bool share_of(const AttendArgs& a, int h, int slot, S
   for (int s0 = 0;; s0 += 64) {
     const int shares = blocks <= per ? 1 : (blocks + per - 1) / per;
     const int mine = tiles * shares;
-    const int upto = wave_incl_scan(mine);
+    const int upto = wave_incl_scan_dpp(mine);
     const unsigned long long past = __ballot(before + upto > slot);
     if (past) {
       const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)past) - 1);
@@ -440,14 +485,16 @@ template <int D, int FMT, int R>
 struct WaveRows {
   static constexpr int PARTS = 64 / R;          // lanes that share a row
   static constexpr int MINE = KB / PARTS;       // a lane's keys of a block
-  static constexpr int GROUPS = KB / R;         // products of R keys
+  static constexpr int STEPS = R == 16 ? 1 : 2; // a block of keys is taken in this many steps (32 rows: registers)
+  static constexpr int GROUPS = KB / R / STEPS; // products of R keys in a step
   static constexpr int SEG = 16 * PARTS;        // dims that one 16-byte load of every part covers
   static constexpr int NT = D / R;              // R-dim tiles of O^T
   static constexpr int NI = R * R / 64;         // accumulator values of a lane
   static constexpr float P_SCALE = 0x1p11f, SLACK = 4.f;
   typedef __attribute__((ext_vector_type(NI))) float acc_t;
   typedef u32x4_t kcodes_t[GROUPS][D / SEG];
-  typedef u32x4_t vcodes_t[NT][MINE / 16];
+  static constexpr int KEYS = MINE / STEPS;     // a lane's keys of a step: 16
+  typedef u32x4_t vcodes_t[NT];
 
   acc_t o[NT];
   float m, l;
@@ -492,26 +539,25 @@ struct WaveRows {
 
   // A block's codes through a buffer resource of its size: the address of a load is a scalar base, one lane
   // offset and a scalar or literal one.  (By pointers the compiler carries 64-bit lane addresses and spills.)
-  static __device__ __forceinline__ void load_k(const uint8_t* kb, int lane, kcodes_t& kc) {
+  static __device__ __forceinline__ void load_k(const uint8_t* kb, int step, int lane, kcodes_t& kc) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)kb, 0, KB * D, BUFFER_CONFIG);
+    if constexpr (R * D > 4096) lane = lane_again();      // the offset made here: registers less to keep
     const int off = key_of(lane % R, 0) * D + (lane / R) * 16;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
       for (int j = 0; j < D / SEG; ++j)
-        kc[g][j] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + j * SEG, key_of(0, g) * D, 0);
+        kc[g][j] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, key_of(0, step * GROUPS + g) * D + j * SEG, 0);
   }
-  static __device__ __forceinline__ void load_v(const uint8_t* vb, int lane, vcodes_t& vc) {
+  static __device__ __forceinline__ void load_v(const uint8_t* vb, int step, int lane, vcodes_t& vc) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)vb, 0, KB * D, BUFFER_CONFIG);
+    if constexpr (R * D > 4096) lane = lane_again();
     const int off = (lane % R) * KB + (lane / R) * MINE;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int x = 0; x < MINE / 16; ++x)
-        vc[t][x] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + x * 16, t * R * KB, 0);
+    for (int t = 0; t < NT; ++t) vc[t] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, t * R * KB + step * KEYS, 0);
   }
 
-  // scores of a block's keys, times ks; q(j, x) gives the rows' pieces
+  // scores of a step's keys, times ks; q(j, x) gives the rows' pieces
   template <class Q>
   static __device__ __forceinline__ void scores(const kcodes_t& kc, Q&& q, float ks, acc_t (&sc)[GROUPS]) {
 #pragma unroll
@@ -538,25 +584,23 @@ struct WaveRows {
       for (int i = 0; i < NI; ++i) sc[g][i] *= ks;
   }
 
-  // a block's scores to probabilities p (fp16, with the values' scale), the state moved on.  seen: how
-  // many of its keys the lane's row sees (all: every row every one).  Returns the lane's sum.
-  __device__ __forceinline__ float softmax(acc_t (&sc)[GROUPS], float vs, int seen, bool all, int lane,
-                                           u32x4_t (&p)[MINE / 8]) {
-    const int part = lane / R;
+  // a step's scores to probabilities p (fp16, with the values' scale), the state moved on.  seen: how
+  // many of the lane's keys of the step its row sees (all: every row every one).  Returns the lane's sum.
+  __device__ __forceinline__ float softmax(acc_t (&sc)[GROUPS], float vs, int seen, bool all, u32x4_t (&p)[KEYS / 8]) {
     if (!all) {
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-          if (part * MINE + g * NI + i >= seen) sc[g][i] = -INFINITY;
+          if (g * NI + i >= seen) sc[g][i] = -INFINITY;
     }
     float top = -INFINITY;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
       for (int i = 0; i < NI; ++i) top = fmaxf(top, sc[g][i]);
-    if constexpr (R == 16) top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if constexpr (R == 16) top = max16(top);
+    top = max32(top);
     // the reference maximum moves only when a row has gone 2^SLACK above it, the reference
     // scale when a block's is larger
     if (__ballot(top > m + SLACK || fabsf(vs) > v_ref)) {
@@ -585,37 +629,33 @@ struct WaveRows {
     const float pv = v_ref > 0.f ? vs / v_ref * P_SCALE : vs * 0.f;       // a NaN scale stays one
     float sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < MINE / 2; ++x) {
+    for (int x = 0; x < KEYS / 2; ++x) {
       const int i0 = 2 * x, i1 = 2 * x + 1;
       const float p0 = __builtin_amdgcn_exp2f(sc[i0 / NI][i0 % NI] - ref);
       const float p1 = __builtin_amdgcn_exp2f(sc[i1 / NI][i1 % NI] - ref);
       sum += p0 + p1;
       // an unseen key's product is 0 whatever the scale
-      const bool h0 = !all && part * MINE + i0 >= seen, h1 = !all && part * MINE + i1 >= seen;
+      const bool h0 = !all && i0 >= seen, h1 = !all && i1 >= seen;
       p[x / 4][x % 4] = pack2h(h0 ? 0.f : p0 * pv, h1 ? 0.f : p1 * pv);
     }
     l += sum;
     return sum;
   }
 
-  // filled: how many of the block's keys are there
-  __device__ __forceinline__ void values(vcodes_t& vc, const u32x4_t (&p)[MINE / 8], int filled, int lane) {
-    if (filled < KB) {
+  // filled: how many of the lane's keys of the step are there (whole: all of every lane)
+  __device__ __forceinline__ void values(vcodes_t& vc, const u32x4_t (&p)[KEYS / 8], int filled, bool whole) {
+    if (!whole) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int x = 0; x < MINE / 16; ++x) vc[t][x] = clear_past(vc[t][x], filled - ((lane / R) * MINE + x * 16));
+      for (int t = 0; t < NT; ++t) vc[t] = clear_past(vc[t], filled);
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int x = 0; x < MINE / 16; ++x) {
-        u32x4_t w = vc[t][x];
-        asm volatile("" : "+v"(w));
-        o[t] = mfma(decode8h<FMT>(w.x, w.y), as_f16x8(p[2 * x]), o[t]);
-        o[t] = mfma(decode8h<FMT>(w.z, w.w), as_f16x8(p[2 * x + 1]), o[t]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int t = 0; t < NT; ++t) {
+      u32x4_t w = vc[t];
+      asm volatile("" : "+v"(w));
+      o[t] = mfma(decode8h<FMT>(w.x, w.y), as_f16x8(p[0]), o[t]);
+      o[t] = mfma(decode8h<FMT>(w.z, w.w), as_f16x8(p[1]), o[t]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 
   // the row's sum over its lanes, and O as the wave's own result (normalised before it gets the values'
@@ -648,17 +688,16 @@ struct LaneRow {
     head = h * a.g + r % a.g;
     there = r < a.tile_queries * a.g && qi < x.n;
     token = x.row0 + qi;
-    vis = there ? x.held - x.n + qi + 1 : 0;
-    vis = vis < 0 ? 0 : vis;
-    vis_most = vis;
-    vis_least = there ? vis : 0x7fffffff;
-#pragma unroll
-    for (int y = 1; y < R; y <<= 1) {
-      vis_most = max(vis_most, __shfl_xor(vis_most, y, 64));
-      vis_least = min(vis_least, __shfl_xor(vis_least, y, 64));
-    }
-    vis_most = __builtin_amdgcn_readfirstlane(vis_most);
-    vis_least = __builtin_amdgcn_readfirstlane(vis_least);
+    auto sees = [&](int row) {
+      const int v = x.held - x.n + x.q0 + row / a.g + 1;
+      return v < 0 ? 0 : v;
+    };
+    vis = there ? sees(r) : 0;
+    // the wave's rows are R in a row: the last one that is there sees the most, the first the least
+    const int left = (x.n - x.q0 < a.tile_queries ? x.n - x.q0 : a.tile_queries) * a.g;
+    const int first = __builtin_amdgcn_readfirstlane(row), last = first + R < left ? first + R - 1 : left - 1;
+    vis_most = first < left ? sees(last) : 0;
+    vis_least = first < left ? sees(first) : 0x7fffffff;
   }
 
   // four dims of the row's result: to out, or where its shares are joined
@@ -688,13 +727,13 @@ struct LaneRow {
 // wave, the waves joined through LDS.  The codes go from memory to the registers that the products read,
 // the next block's on their way while this one's are used; no barrier and no LDS traffic but the queries'.
 template <int D, int FMT, int R>
-__global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_keys_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256, 2) void attend_keys_kernel(AttendArgs a) {
   using W = WaveRows<D, FMT, R>;
   constexpr int TILE = W::NT * W::NI * 64;          // floats of a wave's O
   constexpr int PIECES = D / W::SEG * 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_keys[];
-  float* fold = reinterpret_cast<float*>(smem_keys);
-  __shared__ u32x4_t sq[PIECES * 64];
+  float* fold = reinterpret_cast<float*>(smem_keys);      // after the keys
+  u32x4_t* sq = reinterpret_cast<u32x4_t*>(smem_keys);    // before
   __shared__ float sm[4 * 64], sl[4 * 64];
   const sbsa_cache8& c = a.c;
   const int lane = threadIdx.x & 63;
@@ -705,7 +744,6 @@ __global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_keys_
   LaneRow<R> r;
   r.find(a, h, sh, lane % R);
   const bf16_t* qrow = r.there ? a.q + r.token * a.q_st + r.head * a.q_sh : nullptr;
-  for (int i = wave; i < PIECES; i += 4) sq[i * 64 + lane] = W::query_piece(qrow, i >> 1, i & 1, lane);
 
   W w;
   w.start();
@@ -715,71 +753,125 @@ __global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_keys_
   const uint8_t* codes_v = (const uint8_t*)c.codes_v + base * KB * D;
   const int first = sh.lo + wave;
   const int count = sh.hi > first ? (sh.hi - first + 3) / 4 : 0;
-  // the places and scales of the wave's next 64 blocks, one per lane
-  int place = 0;
-  float ks = 0.f, vs = 0.f;
-  auto fetch = [&](int i0) {
+  // the places and scales of the wave's next 64 blocks: fetched by a lane each, kept in LDS
+  __shared__ int s_place[4 * 64];
+  __shared__ float s_ks[4 * 64], s_vs[4 * 64];
+  auto fetch = [&](int i0, auto&& then) {           // then: what goes on as soon as the places are there
     const int b = first + 4 * (i0 + lane);
-    place = 0;
+    int place = 0;
     if (b < sh.hi) {
       place = (int)(place_of(c, row, b) - base);
-      ks = c.scales[base + place] * a.scale_log2;
-      vs = c.scales[heads * c.num_blocks + base + place];
+      s_place[wave * 64 + lane] = place;
     }
+    __builtin_amdgcn_wave_barrier();
+    then();
+    if (b < sh.hi) {
+      s_ks[wave * 64 + lane] = c.scales[base + place] * a.scale_log2;
+      s_vs[wave * 64 + lane] = c.scales[heads * c.num_blocks + base + place];
+    }
+    __builtin_amdgcn_wave_barrier();
+  };
+  auto place_at = [&](int i) {                      // in bytes of codes
+    return (int64_t)__builtin_amdgcn_readfirstlane(s_place[wave * 64 + (i & 63)]) * (KB * D);
   };
   typename W::kcodes_t kc;
   typename W::vcodes_t vc;
   if (count > 0) {
-    fetch(0);
-    const int64_t at = (int64_t)__builtin_amdgcn_readlane(place, 0) * (KB * D);
-    W::load_k(codes_k + at, lane, kc);
-    W::load_v(codes_v + at, lane, vc);
+    fetch(0, [&] {
+      const int64_t at = place_at(0);
+      W::load_k(codes_k + at, 0, lane, kc);
+      W::load_v(codes_v + at, 0, lane, vc);
+    });
   }
+  for (int i = wave; i < PIECES; i += 4) sq[i * 64 + lane] = W::query_piece(qrow, i >> 1, i & 1, lane);
   __syncthreads();                                  // the queries are in LDS
+  float sum_m = 0.f, sum = 0.f;                     // the block's sum so far, at reference maximum sum_m
   for (int i = 0; i < count; ++i) {
     const int b = first + 4 * i;
-    const float ksi = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(ks), i & 63));
-    const float vsi = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(vs), i & 63));
-    if (((i + 1) & 63) == 0) fetch(i + 1);
-    const int64_t at = (int64_t)__builtin_amdgcn_readlane(place, (i + 1) & 63) * (KB * D);
-    typename W::acc_t sc[W::GROUPS];
-    W::scores(kc, [&](int j, int x) { return sq[(2 * j + x) * 64 + lane]; }, ksi, sc);
-    if (i + 1 < count) W::load_k(codes_k + at, lane, kc);
-    u32x4_t p[W::MINE / 8];
-    float sum = w.softmax(sc, vsi, r.vis - b * KB, (b + 1) * KB <= r.vis_least, lane, p);
-    if (a.part_w) {
-      // the block's share of each row's attention, for the blocks' weights
-      if constexpr (R == 16) sum += __shfl_xor(sum, 16, 64);
-      sum += __shfl_xor(sum, 32, 64);
-      if (r.there && lane < R)
-        a.part_w[(r.token * a.hq + r.head) * c.num_blocks + b] = f32x2_t{w.m, sum};
+    const float ksi = uniform(s_ks[wave * 64 + (i & 63)]), vsi = uniform(s_vs[wave * 64 + (i & 63)]);
+    const int64_t here = place_at(i);
+    if (((i + 1) & 63) == 0) fetch(i + 1, [] {});
+    const int64_t next = i + 1 < count ? place_at(i + 1) : 0;
+#pragma unroll
+    for (int step = 0; step < W::STEPS; ++step) {
+      // what is loaded next: this block's next step, or the next block's first
+      const bool more = step + 1 < W::STEPS || i + 1 < count;
+      const int64_t at = step + 1 < W::STEPS ? here : next;
+      const int then = (step + 1) % W::STEPS, mine = (lane / R) * W::MINE + step * W::KEYS;
+      typename W::acc_t sc[W::GROUPS];
+      const int own = R * D > 4096 ? lane_again() : lane;       // a reload from scratch would wait for every load
+      W::scores(kc, [&](int j, int x) { return sq[(2 * j + x) * 64 + own]; }, ksi, sc);
+      if (more) W::load_k(codes_k + at, then, lane, kc);
+      u32x4_t p[W::KEYS / 8];
+      const float part_sum = w.softmax(sc, vsi, r.vis - b * KB - mine, (b + 1) * KB <= r.vis_least, p);
+      if (a.part_w) {
+        // the block's share of each row's attention, for the blocks' weights
+        sum = step == 0 ? part_sum : sum * (sum_m == w.m ? 1.f : __builtin_amdgcn_exp2f(sum_m - w.m)) + part_sum;
+        sum_m = w.m;
+        if (step + 1 == W::STEPS) {
+          if constexpr (R == 16) sum += __shfl_xor(sum, 16, 64);
+          sum += __shfl_xor(sum, 32, 64);
+          if (r.there && lane < R)
+            a.part_w[(r.token * a.hq + r.head) * c.num_blocks + b] = f32x2_t{w.m, sum};
+        }
+      }
+      w.values(vc, p, sh.held - b * KB - mine, sh.held - b * KB >= KB);
+      if (more) W::load_v(codes_v + at, then, lane, vc);
+      asm volatile("" ::: "memory");                // the queries stay in LDS, not in registers
     }
-    w.values(vc, p, sh.held - b * KB, lane);
-    if (i + 1 < count) W::load_v(codes_v + at, lane, vc);
-    asm volatile("" ::: "memory");                  // the queries stay in LDS, not in registers
   }
   w.total();
+  // The waves' results joined.  Where all four do not fit LDS twice on a compute unit (32 rows of 256 dims),
+  // the odd waves' go into the even ones' first.
+  constexpr int LEFT = R * D > 4096 ? 2 : 4;        // results that the last step joins
+  auto leave = [&](int at) {
 #pragma unroll
-  for (int t = 0; t < W::NT; ++t)
+    for (int t = 0; t < W::NT; ++t)
 #pragma unroll
-    for (int i = 0; i < W::NI; ++i) fold[wave * TILE + (t * W::NI + i) * 64 + lane] = w.o[t][i];
-  sm[wave * 64 + lane] = w.m;
-  sl[wave * 64 + lane] = w.l;
+      for (int i = 0; i < W::NI; ++i) fold[at * TILE + (t * W::NI + i) * 64 + lane] = w.o[t][i];
+    sm[at * 64 + lane] = w.m;
+    sl[at * 64 + lane] = w.l;
+  };
+  if constexpr (LEFT == 2) {
+    __syncthreads();                                // the queries' place in LDS is used again
+    if (wave & 1) leave(wave >> 1);
+    __syncthreads();
+    if (!(wave & 1)) {
+      const int at = wave >> 1;
+      const float m1 = sm[at * 64 + lane], l1 = sl[at * 64 + lane];
+      const float to = fmaxf(w.m, m1), ref = to == -INFINITY ? 0.f : to;
+      float f0 = w.l * __builtin_amdgcn_exp2f(w.m - ref), f1 = l1 * __builtin_amdgcn_exp2f(m1 - ref);
+      w.m = to;
+      w.l = f0 + f1;
+      const float inv = w.l == 0.f ? 0.f : 1.f / w.l;
+      f0 *= inv;
+      f1 *= inv;
+#pragma unroll
+      for (int t = 0; t < W::NT; ++t)
+#pragma unroll
+        for (int i = 0; i < W::NI; ++i)
+          w.o[t][i] = w.o[t][i] * f0 + fold[at * TILE + (t * W::NI + i) * 64 + lane] * f1;
+      leave(at);                                    // each lane into the place that it read
+    }
+  } else {
+    __syncthreads();
+    leave(wave);
+  }
   __syncthreads();
   // each wave joins a quarter of the dims
-  float top = -INFINITY, f[4], total = 0.f;
+  float top = -INFINITY, f[LEFT], total = 0.f;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) top = fmaxf(top, sm[x * 64 + lane]);
+  for (int x = 0; x < LEFT; ++x) top = fmaxf(top, sm[x * 64 + lane]);
   const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
+  for (int x = 0; x < LEFT; ++x) {
     f[x] = sl[x * 64 + lane] * __builtin_amdgcn_exp2f(sm[x * 64 + lane] - ref);
     total += f[x];
   }
   if (!r.there) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-  for (int x = 0; x < 4; ++x) f[x] *= inv;
+  for (int x = 0; x < LEFT; ++x) f[x] *= inv;
   constexpr int OWN = W::NT / 4;
 #pragma unroll
   for (int tt = 0; tt < OWN; ++tt) {
@@ -790,7 +882,9 @@ __global__ __launch_bounds__(256, R == 32 && D == 256 ? 1 : 2) void attend_keys_
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int at = (t * W::NI + 4 * q + i) * 64 + lane;
-        v[i] = (fold[at] * f[0] + fold[TILE + at] * f[1]) + (fold[2 * TILE + at] * f[2] + fold[3 * TILE + at] * f[3]);
+        float y = fold[at] * f[0] + fold[TILE + at] * f[1];
+        if constexpr (LEFT == 4) y += fold[2 * TILE + at] * f[2] + fold[3 * TILE + at] * f[3];
+        v[i] = y;
       }
       r.store(a, h, slot, sh, D, W::dim_of(t, q, lane), v);
     }
@@ -816,11 +910,6 @@ __device__ __forceinline__ void lds_load16(u32x4_t rsrc, uint32_t lds_addr, uint
                :
                : "s"(lds_addr), "v"(voffset), "s"(rsrc)
                : "memory", "m0");
-}
-
-// a value that is the same in every lane, in a scalar register
-__device__ __forceinline__ float uniform(float v) {
-  return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(v)));
 }
 
 // A load through the scalar cache, by an address that is the same in every lane (of memory that no block of the launch writes).
@@ -867,6 +956,7 @@ template <int D, int FMT>
 __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
   using T = RowsTile<D, FMT>;
   constexpr int NT = D / 32, STEPS = D / 32;
+  constexpr int K_AHEAD = 2, V_AHEAD = 2;
   constexpr float P_LOG2 = 11.f, SLACK = 4.f;          // as in WaveRows
   __shared__ __attribute__((aligned(16))) unsigned char tile[2][2 * T::BYTES];
   const sbsa_cache8& c = a.c;
@@ -965,19 +1055,29 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
       auto query = [&](int j, int x) {
         return j < KEPT ? q[j < KEPT ? j : 0][x] : as_bf16x8(sq[(2 * (j - KEPT) + x) * 256 + threadIdx.x]);
       };
-      // a fragment one step ahead; further, and the compiler runs out of registers
       auto key_piece = [&](int j) {
         return *reinterpret_cast<const u32x4_t*>(&tile[0][0] + (kat ^ (32u * j)) + 16 * g * D);
       };
-      u32x4_t ahead = key_piece(0);
+      auto value_piece = [&](int t) {
+        return *reinterpret_cast<const u32x4_t*>(&tile[0][0] + (vat ^ (16u * g)) + t * 32 * KB);
+      };
+      // pieces K_AHEAD and V_AHEAD steps ahead, the values' first ones under the softmax; further, and the
+      // compiler runs out of registers
+      __builtin_amdgcn_s_setprio(1);                   // the products before the other block's softmax: 2 %
+      u32x4_t kp[K_AHEAD], vp[V_AHEAD];
+#pragma unroll
+      for (int j = 0; j < K_AHEAD; ++j) kp[j] = key_piece(j);
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {
-        const u32x4_t w = ahead;
-        if (j + 1 < STEPS) ahead = key_piece(j + 1);
+        const u32x4_t w = kp[j % K_AHEAD];
         sc = W::mfma(decode8<FMT>(w.x, w.y), query(j, 0), sc);
         sc = W::mfma(decode8<FMT>(w.z, w.w), query(j, 1), sc);
+        if (j + K_AHEAD < STEPS) kp[j % K_AHEAD] = key_piece(j + K_AHEAD);
         __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int t = 0; t < V_AHEAD; ++t) vp[t] = value_piece(t);
+      __builtin_amdgcn_s_setprio(0);
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -985,7 +1085,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
         if (!all && part * 32 + g * 16 + i >= seen) sc[i] = -INFINITY;
         top = fmaxf(top, sc[i]);
       }
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      top = max32(top);
       if (__ballot(top > m + SLACK)) {
         if (__ballot(top == INFINITY)) {               // as in WaveRows
 #pragma unroll
@@ -1016,19 +1116,17 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
         p[i / 8][i / 2 % 4] = pack2h(p0, p1);
       }
       l += sum * drop;
-      auto value_piece = [&](int t) {
-        return *reinterpret_cast<const u32x4_t*>(&tile[0][0] + (vat ^ (16u * g)) + t * 32 * KB);
-      };
-      ahead = value_piece(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        u32x4_t w = ahead;
-        if (t + 1 < NT) ahead = value_piece(t + 1);
+        u32x4_t w = vp[t % V_AHEAD];
         if (!whole) w = clear_past(w, sh.held - b * KB - (part * 32 + g * 16));
         o[t] = W::mfma(decode8h<FMT>(w.x, w.y), as_f16x8(p[0]), o[t]);
         o[t] = W::mfma(decode8h<FMT>(w.z, w.w), as_f16x8(p[1]), o[t]);
+        if (t + V_AHEAD < NT) vp[t % V_AHEAD] = value_piece(t + V_AHEAD);
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
   }
   l += __shfl_xor(l, 32, 64);
@@ -1047,13 +1145,42 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
 }
 
 // The shares joined.  The first blocks of the grid each take 64 dims of a row, 16 threads to a share's 64 dims and every
-// 16th share to each; with part_w the others take 256 blocks of keys of a (sequence, head) and
+// 16th share to each (FEW: the 64 dims of 16 rows, every share of a row to its 16 threads); with part_w the others take 256 blocks of keys of a (sequence, head) and
 // add up what the rows left for each of them.
-template <int D>
+template <int D, bool FEW>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks) {
   const int tid = threadIdx.x, lane = tid & 63;
   const sbsa_cache8& c = a.c;
-  if ((int)blockIdx.x < join_blocks) {
+  if (FEW && (int)blockIdx.x < join_blocks) {
+    const int64_t unit = (int64_t)blockIdx.x * 16 + (tid >> 4), row = unit / (D / 64), token = row / a.hq;
+    const int d = (int)(unit % (D / 64)) * 64 + (tid & 15) * 4, head = (int)(row % a.hq);
+    if (token >= a.tokens || (a.offsets && (token < a.offsets[0] || token >= a.offsets[c.num_seqs]))) return;
+    const i32x4_t where = a.where[row];
+    if (where.y == 1) return;
+    const int64_t at = ((int64_t)(head / a.g) * a.slots + where.x) * a.tile_rows + where.z;
+    const f32x2_t* ml = a.part_ml + at;
+    float top = -INFINITY, total = 0.f;
+    for (int x = 0; x < where.y; ++x) top = fmaxf(top, ml[(int64_t)x * a.tile_rows].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int x = 0; x < where.y; ++x) {
+      const f32x2_t v = ml[(int64_t)x * a.tile_rows];
+      total += v.y * __builtin_amdgcn_exp2f(v.x - ref);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    for (int x = 0; x < where.y; ++x) {
+      const f32x2_t v = ml[(int64_t)x * a.tile_rows];
+      const f32x4_t o = *reinterpret_cast<const f32x4_t*>(a.part_o + (at + (int64_t)x * a.tile_rows) * D + d);
+      acc += o * (v.y * __builtin_amdgcn_exp2f(v.x - ref) * inv);
+    }
+    u32x2_t w;
+    w.x = pack2bf(acc.x, acc.y);
+    w.y = pack2bf(acc.z, acc.w);
+    *reinterpret_cast<u32x2_t*>(a.out + token * a.o_st + head * a.o_sh + d) = w;
+    if (d == 0) finish_row(a, row, top, total);
+    return;
+  }
+  if (!FEW && (int)blockIdx.x < join_blocks) {
     const int64_t row = blockIdx.x / (D / 64);
     const int dims = (int)(blockIdx.x % (D / 64)) * 64;
     const int64_t token = row / a.hq;
@@ -1152,8 +1279,9 @@ __global__ __launch_bounds__(256) void weigh_kernel(AttendArgs a) {
   const int held = held_of(c, sh);
   if (n == 0 || b * KB >= held) return;
   const int64_t place = place_of(c, sh, b);
-  typename W::kcodes_t kc;
-  W::load_k((const uint8_t*)c.codes_k + place * (KB * D), lane, kc);
+  typename W::kcodes_t kc[W::STEPS];
+#pragma unroll
+  for (int step = 0; step < W::STEPS; ++step) W::load_k((const uint8_t*)c.codes_k + place * (KB * D), step, lane, kc[step]);
   const float ks = c.scales[place] * a.scale_log2;
   // the first row that sees the block's first key
   int first = b * KB - (held - n);
@@ -1168,13 +1296,18 @@ __global__ __launch_bounds__(256) void weigh_kernel(AttendArgs a) {
     const bf16_t* qrow = there ? a.q + (row0 + qi) * a.q_st + head * a.q_sh : nullptr;
     const f32x2_t none = {0.f, 0.f};
     const f32x2_t all = there ? a.row_ml[(row0 + qi) * a.hq + head] : none;
-    typename W::acc_t sc[W::GROUPS];
-    W::scores(kc, [&](int j, int x) { return W::query_piece(qrow, j, x, lane); }, ks, sc);
 #pragma unroll
-    for (int g = 0; g < W::GROUPS; ++g)
+    for (int step = 0; step < W::STEPS; ++step) {
+      typename W::acc_t sc[W::GROUPS];
+      W::scores(kc[step], [&](int j, int x) { return W::query_piece(qrow, j, x, lane); }, ks, sc);
 #pragma unroll
-      for (int i = 0; i < W::NI; ++i)
-        sum += (lane / 32) * W::MINE + g * W::NI + i < seen ? __builtin_amdgcn_exp2f(fminf(sc[g][i], FLT_MOST) - all.x) * all.y : 0.f;
+      for (int g = 0; g < W::GROUPS; ++g)
+#pragma unroll
+        for (int i = 0; i < W::NI; ++i)
+          sum += (lane / 32) * W::MINE + step * W::KEYS + g * W::NI + i < seen
+                     ? __builtin_amdgcn_exp2f(fminf(sc[g][i], FLT_MOST) - all.x) * all.y
+                     : 0.f;
+    }
   }
   sum = wave_sum(sum);
   if (lane == 0) c.weights[sh * c.num_blocks + b] += sum;
@@ -1340,7 +1473,12 @@ bool bad_rows(const void* p, int64_t st, int64_t sh) { return !p || (uintptr_t)p
 
 template <int D, int FMT>
 void launch_append(const AppendArgs& a, dim3 grid, hipStream_t stream) {
-  hipLaunchKernelGGL((append_kernel<D, FMT>), grid, dim3(256), 0, stream, a);
+  if (grid.x == 2) {
+    hipLaunchKernelGGL((append_kernel<D, FMT, true>), grid, dim3(256), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((append_kernel<D, FMT, false>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((append_end_kernel<D>), dim3(grid.y, grid.z), dim3(256), 0, stream, a);
+  }
 }
 
 // How a call's rows go over the grid.
@@ -1365,7 +1503,8 @@ AttendPlan plan_attend(const sbsa_cache8* c, int num_q_heads, int64_t tokens, in
   // tile of few rows or of few keys stays whole, which saves the join.
   const int64_t heads = c->num_kv_heads;
   p.target = 0;
-  if (tiles * heads < 512 && c->num_blocks > 16) p.target = (int)(512 / heads < 1 ? 1 : 512 / heads);
+  const int64_t want = p.keys || tiles * heads < 512 ? 512 : 1024;
+  if (tiles * heads < want && c->num_blocks > 16) p.target = (int)(want / heads < 1 ? 1 : want / heads);
   p.slots = tiles + p.target;
   return p;
 }
@@ -1390,7 +1529,7 @@ AttendSpace attend_space(const AttendPlan& p, const sbsa_cache8* c, int64_t toke
 
 template <int D, int FMT, int R>
 bool launch_keys(const AttendArgs& a, dim3 grid, hipStream_t stream) {
-  constexpr int lds = 4 * R * D * (int)sizeof(float);
+  constexpr int lds = (R * D > 4096 ? 2 : 4) * R * D * (int)sizeof(float);
   if (lds > 48 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(attend_keys_kernel<D, FMT, R>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
     return false;
@@ -1406,9 +1545,15 @@ bool launch_attend(const AttendArgs& a, const AttendPlan& p, int accumulate, hip
   else if (!(p.tile_rows == 16 ? launch_keys<D, FMT, 16>(a, grid, stream) : launch_keys<D, FMT, 32>(a, grid, stream)))
     return false;
   if (p.target) {
-    const int64_t join = a.tokens * a.hq * (D / 64);
+    // few shares of many rows, or many of few: 512 blocks of 16 row pieces fill the card (a 512-token chunk at 16000 keys
+    // 177 us so, 203 with a block per piece; 16 sequences' tokens at 8192 keys 42 so, 36 with a block per piece)
+    const bool few = a.tokens * a.hq * (D / 64) >= 8192;
+    const int64_t join = few ? (a.tokens * a.hq * (D / 64) + 15) / 16 : a.tokens * a.hq * (D / 64);
     const int64_t weigh = a.part_w ? (int64_t)((a.c.num_blocks + 255) / 256) * a.c.num_kv_heads * a.c.num_seqs : 0;
-    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(join + weigh)), dim3(256), 0, stream, a, (int)join);
+    if (few)
+      hipLaunchKernelGGL((join_kernel<D, true>), dim3((unsigned)(join + weigh)), dim3(256), 0, stream, a, (int)join);
+    else
+      hipLaunchKernelGGL((join_kernel<D, false>), dim3((unsigned)(join + weigh)), dim3(256), 0, stream, a, (int)join);
   }
   if (accumulate && !a.part_w)
     hipLaunchKernelGGL((weigh_kernel<D, FMT>),
@@ -1435,7 +1580,7 @@ extern "C" int sbsa_cache8_append(const sbsa_cache8* cache, const void* k, int64
   int64_t most = offsets ? (max_rows < 1 || max_rows > tokens ? tokens : max_rows) : a.uniform;
   int64_t blocks = most < 1 ? 1 : (most + KB - 2) / KB + 1;
   if (blocks > cache->num_blocks) blocks = cache->num_blocks;
-  const dim3 grid((unsigned)blocks, (unsigned)cache->num_kv_heads, (unsigned)cache->num_seqs);
+  const dim3 grid((unsigned)(2 * blocks), (unsigned)cache->num_kv_heads, (unsigned)cache->num_seqs);
   if (cache->head_dim == 128)
     cache->format == SBSA_CACHE8_E4M3 ? launch_append<128, SBSA_CACHE8_E4M3>(a, grid, stream)
                                       : launch_append<128, SBSA_CACHE8_INT8>(a, grid, stream);

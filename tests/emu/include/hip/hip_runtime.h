@@ -190,6 +190,23 @@ __forceinline__ u32pair permlane32_swap(uint32_t vdst, uint32_t vsrc, bool, bool
   }
   return r;
 }
+// v_permlane16_swap: the odd rows of 16 of vdst swapped with the even rows before them of vsrc
+__forceinline__ u32pair permlane16_swap(uint32_t vdst, uint32_t vsrc, bool, bool) {
+  struct Two {
+    uint32_t v[2];
+  } both{{vdst, vsrc}};
+  const auto all = gather(both);
+  const int l = lane();
+  u32pair r;
+  if (l & 16) {
+    r.v[0] = all[l - 16].v[1];
+    r.v[1] = all[l].v[1];
+  } else {
+    r.v[0] = all[l].v[0];
+    r.v[1] = all[l + 16].v[0];
+  }
+  return r;
+}
 // ds_read_b64_tr_b16: lane 16 g + i receives element i % 4 of the 64-bit words
 // addressed by lanes 16 g + i / 4 + 4 e, e = 0..3
 __forceinline__ emu_s16x4_t ds_read_tr16_b64(const void* p) {
@@ -363,6 +380,9 @@ __forceinline__ VC mfma_f16(V8 a, V8 b, VC c) {
 }
 }  // namespace emu
 #define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, hi) emu::cvt_pk_f16_fp8((w), (s), (hi))
+#define __builtin_amdgcn_mbcnt_lo(m, x) (0u)
+#define __builtin_amdgcn_mbcnt_hi(m, x) ((unsigned)emu::lane())
+#define __builtin_amdgcn_permlane16_swap(a, b, f, c) emu::permlane16_swap((a), (b), (f), (c))
 #define __builtin_amdgcn_perm(a, b, sel) emu::perm((a), (b), (sel))
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) emu::mfma_f16<32>((a), (b), (c))
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, x, y, z) emu::mfma_f16<16>((a), (b), (c))
