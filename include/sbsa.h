@@ -487,7 +487,7 @@ typedef struct sbsa_cache8 {
 } sbsa_cache8;
 
 /* New rows behind each sequence's tokens.  k, v [tokens, Hkv, dim] bf16; sequence s has rows
- * offsets[s] .. offsets[s+1] (device int32 [S+1]; null: tokens / S rows each).  start (device int32
+ * offsets[s] .. offsets[s+1] (device int32 [S+1], ascending; null: tokens / S rows each).  start (device int32
  * [S], or null: the lengths): the rows go to start[s] onwards and the sequence ends behind them
  * (start is at most the length; no rows: the sequence is cut there).  Each touched block is quantised
  * whole from its bf16 rows: the new ones, and the earlier ones from tail, or from their codes where tail

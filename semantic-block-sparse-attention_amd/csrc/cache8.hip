@@ -904,9 +904,10 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 
 // 16 bytes per lane from memory straight to LDS, lane l's at lds_addr + 16 l.  In assembly, because the compiler waits for
 // the builtin's loads before any LDS read that it cannot tell apart; the kernel waits (vmcnt) before the
-// barrier that publishes a tile.  M0 holds the LDS base; nothing else in the kernel uses it.
+// barrier that publishes a tile.  M0 holds the LDS base (a wait state lies between its write and its use); nothing else in the
+// kernel uses it.
 __device__ __forceinline__ void lds_load16(u32x4_t rsrc, uint32_t lds_addr, uint32_t voffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds_addr), "v"(voffset), "s"(rsrc)
                : "memory", "m0");
@@ -1043,9 +1044,17 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] *= f;
     }
-    // in (0, 1], or NaN; below 2^-60 fp16 has nothing left of the block's values, but its keys still count
-    float ratio = v_ref > 0.f ? vs / v_ref : vs - vs + 1.f;
+    // in (0, 1]; below 2^-60 fp16 has nothing left of the block's values, but its keys still count (as do those of
+    // a block whose values are not finite)
+    float ratio = v_ref > 0.f && vs == vs ? vs / v_ref : 1.f;
     ratio = ratio < 0x1p-60f ? 0x1p-60f : ratio;
+    if (vs != vs) {                                    // NaN to every row that sees a value of the block
+      const float none = seen > 0 ? vs : 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] += none;
+    }
     const float lift = uniform(P_LOG2 + __builtin_amdgcn_logf(ratio)), drop = uniform(1.f / (ratio * 2048.f));
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
@@ -1144,6 +1153,11 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
   if (lane < 32) r.store_sum(a, h, slot, sh, m, l);
 }
 
+// Whether a row's shares lie in the workspace.  Rows that no share reached (offsets that do not ascend) have none.
+__device__ __forceinline__ bool shares_fit(const AttendArgs& a, const i32x4_t& w) {
+  return w.x >= 0 && w.y >= 1 && w.y <= a.slots && w.x <= a.slots - w.y && w.z >= 0 && w.z < a.tile_rows;
+}
+
 // The shares joined.  The first blocks of the grid each take 64 dims of a row, 16 threads to a share's 64 dims and every
 // 16th share to each (FEW: the 64 dims of 16 rows, every share of a row to its 16 threads); with part_w the others take 256 blocks of keys of a (sequence, head) and
 // add up what the rows left for each of them.
@@ -1156,7 +1170,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks
     const int d = (int)(unit % (D / 64)) * 64 + (tid & 15) * 4, head = (int)(row % a.hq);
     if (token >= a.tokens || (a.offsets && (token < a.offsets[0] || token >= a.offsets[c.num_seqs]))) return;
     const i32x4_t where = a.where[row];
-    if (where.y == 1) return;
+    if (where.y == 1 || !shares_fit(a, where)) return;
     const int64_t at = ((int64_t)(head / a.g) * a.slots + where.x) * a.tile_rows + where.z;
     const f32x2_t* ml = a.part_ml + at;
     float top = -INFINITY, total = 0.f;
@@ -1187,7 +1201,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks
     const int head = (int)(row % a.hq);
     if (a.offsets && (token < a.offsets[0] || token >= a.offsets[c.num_seqs])) return;
     const i32x4_t where = a.where[row];
-    if (where.y == 1) return;                          // its one share wrote the result
+    if (where.y == 1 || !shares_fit(a, where)) return; // (a single share wrote the result itself)
     __shared__ f32x4_t fold[16 * 16];
     const int64_t at = ((int64_t)(head / a.g) * a.slots + where.x) * a.tile_rows + where.z;
     const f32x2_t* ml = a.part_ml + at;
@@ -1239,6 +1253,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks
     float top = -INFINITY, total = 0.f;
     i32x4_t where = {0, 0, 0, 0};                      // no shares, past the last row
     if (r < (int64_t)n * a.g) where = a.where[(row0 + r / a.g) * a.hq + h * a.g + r % a.g];
+    if (!shares_fit(a, where)) where = i32x4_t{0, 0, 0, 0};
     const f32x2_t* ml = a.part_ml + ((int64_t)h * a.slots + where.x) * a.tile_rows + where.z;
     for (int x = tid & 7; x < where.y; x += 8) top = fmaxf(top, ml[(int64_t)x * a.tile_rows].x);
 #pragma unroll
@@ -1283,31 +1298,52 @@ __global__ __launch_bounds__(256) void weigh_kernel(AttendArgs a) {
 #pragma unroll
   for (int step = 0; step < W::STEPS; ++step) W::load_k((const uint8_t*)c.codes_k + place * (KB * D), step, lane, kc[step]);
   const float ks = c.scales[place] * a.scale_log2;
-  // the first row that sees the block's first key
-  int first = b * KB - (held - n);
-  first = first < 0 ? 0 : first;
-  float sum = 0.f;
-  for (int64_t r0 = (int64_t)first * a.g; r0 < (int64_t)n * a.g; r0 += 32) {
+  // the rows from the first that sees the block's first key, 32 at a time, the next ones on their way meanwhile
+  struct Rows {
+    u32x4_t q[D / W::SEG][2];
+    f32x2_t all;
+    int seen;
+  };
+  auto fetch = [&](int64_t r0, Rows& x) {
     const int64_t r = r0 + lane % 32;
     const bool there = r < (int64_t)n * a.g;
     const int64_t qi = there ? r / a.g : 0;
     const int head = h * a.g + (int)(r % a.g);
-    const int seen = there ? (int)(held - n + qi + 1 - b * KB) : 0;
+    x.seen = there ? (int)(held - n + qi + 1 - b * KB) : 0;
     const bf16_t* qrow = there ? a.q + (row0 + qi) * a.q_st + head * a.q_sh : nullptr;
     const f32x2_t none = {0.f, 0.f};
-    const f32x2_t all = there ? a.row_ml[(row0 + qi) * a.hq + head] : none;
+    x.all = there ? a.row_ml[(row0 + qi) * a.hq + head] : none;
+#pragma unroll
+    for (int j = 0; j < D / W::SEG; ++j)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) x.q[j][y] = W::query_piece(qrow, j, y, lane);
+  };
+  int first = b * KB - (held - n);
+  first = first < 0 ? 0 : first;
+  float sum = 0.f;
+  Rows rows[2];
+  auto add = [&](const Rows& x) {
 #pragma unroll
     for (int step = 0; step < W::STEPS; ++step) {
       typename W::acc_t sc[W::GROUPS];
-      W::scores(kc[step], [&](int j, int x) { return W::query_piece(qrow, j, x, lane); }, ks, sc);
+      W::scores(kc[step], [&](int j, int y) { return x.q[j][y]; }, ks, sc);
 #pragma unroll
       for (int g = 0; g < W::GROUPS; ++g)
 #pragma unroll
         for (int i = 0; i < W::NI; ++i)
-          sum += (lane / 32) * W::MINE + step * W::KEYS + g * W::NI + i < seen
-                     ? __builtin_amdgcn_exp2f(fminf(sc[g][i], FLT_MOST) - all.x) * all.y
+          sum += (lane / 32) * W::MINE + step * W::KEYS + g * W::NI + i < x.seen
+                     ? __builtin_amdgcn_exp2f(fminf(sc[g][i], FLT_MOST) - x.all.x) * x.all.y
                      : 0.f;
     }
+  };
+  const int64_t end = (int64_t)n * a.g;
+  fetch((int64_t)first * a.g, rows[0]);
+  for (int64_t r0 = (int64_t)first * a.g; r0 < end; r0 += 64) {
+    if (r0 + 32 < end) fetch(r0 + 32, rows[1]);
+    add(rows[0]);
+    if (r0 + 32 >= end) break;
+    if (r0 + 64 < end) fetch(r0 + 64, rows[0]);
+    add(rows[1]);
   }
   sum = wave_sum(sum);
   if (lane == 0) c.weights[sh * c.num_blocks + b] += sum;
@@ -1527,6 +1563,21 @@ AttendSpace attend_space(const AttendPlan& p, const sbsa_cache8* c, int64_t toke
   return x;
 }
 
+// Few shares of many rows are joined, or many of few: 512 blocks of 16 row pieces fill the card (a 512-token chunk at
+// 16000 keys 177 us so, 203 with a block per piece; 16 sequences' tokens at 8192 keys 42 so, 36 with a block per piece).
+bool few_shares(const sbsa_cache8* c, int64_t tokens, int num_q_heads) {
+  return tokens * num_q_heads * (c->head_dim / 64) >= 8192;
+}
+
+int64_t join_blocks(const sbsa_cache8* c, int64_t tokens, int num_q_heads) {
+  const int64_t pieces = tokens * num_q_heads * (c->head_dim / 64);
+  return few_shares(c, tokens, num_q_heads) ? (pieces + 15) / 16 : pieces;
+}
+
+int64_t weigh_blocks(const sbsa_cache8* c) {
+  return (int64_t)((c->num_blocks + 255) / 256) * c->num_kv_heads * c->num_seqs;
+}
+
 template <int D, int FMT, int R>
 bool launch_keys(const AttendArgs& a, dim3 grid, hipStream_t stream) {
   constexpr int lds = (R * D > 4096 ? 2 : 4) * R * D * (int)sizeof(float);
@@ -1545,12 +1596,8 @@ bool launch_attend(const AttendArgs& a, const AttendPlan& p, int accumulate, hip
   else if (!(p.tile_rows == 16 ? launch_keys<D, FMT, 16>(a, grid, stream) : launch_keys<D, FMT, 32>(a, grid, stream)))
     return false;
   if (p.target) {
-    // few shares of many rows, or many of few: 512 blocks of 16 row pieces fill the card (a 512-token chunk at 16000 keys
-    // 177 us so, 203 with a block per piece; 16 sequences' tokens at 8192 keys 42 so, 36 with a block per piece)
-    const bool few = a.tokens * a.hq * (D / 64) >= 8192;
-    const int64_t join = few ? (a.tokens * a.hq * (D / 64) + 15) / 16 : a.tokens * a.hq * (D / 64);
-    const int64_t weigh = a.part_w ? (int64_t)((a.c.num_blocks + 255) / 256) * a.c.num_kv_heads * a.c.num_seqs : 0;
-    if (few)
+    const int64_t join = join_blocks(&a.c, a.tokens, a.hq), weigh = a.part_w ? weigh_blocks(&a.c) : 0;
+    if (few_shares(&a.c, a.tokens, a.hq))
       hipLaunchKernelGGL((join_kernel<D, true>), dim3((unsigned)(join + weigh)), dim3(256), 0, stream, a, (int)join);
     else
       hipLaunchKernelGGL((join_kernel<D, false>), dim3((unsigned)(join + weigh)), dim3(256), 0, stream, a, (int)join);
@@ -1612,8 +1659,8 @@ extern "C" int sbsa_cache8_attend(const sbsa_cache8* cache, const void* q, int64
     return SBSA_ERR_UNSUPPORTED;
   if (tokens == 0) return SBSA_OK;
   const AttendPlan p = plan_attend(cache, num_q_heads, tokens, max_rows, offsets != nullptr);
-  if (p.slots >= (1 << 24) ||
-      (int64_t)cache->num_blocks * cache->num_kv_heads * cache->num_seqs / 256 + tokens * num_q_heads * 4 >= (1 << 24))
+  // a grid's threads are below 2^32: fewer than 2^24 blocks of 256
+  if (p.slots >= (1 << 24) || (p.target && join_blocks(cache, tokens, num_q_heads) + weigh_blocks(cache) >= (1 << 24)))
     return SBSA_ERR_UNSUPPORTED;
   const AttendSpace space = attend_space(p, cache, tokens, num_q_heads, accumulate != 0);
   if (workspace_bytes < space.bytes()) return SBSA_ERR_CAPACITY;

@@ -166,6 +166,16 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether [tokens, heads, dim] tensors share memory: as ``overlap``, but columns of one buffer's rows are told apart."""
+    if not overlap(a, b):
+        return False
+    (st, sh, _), size = a.stride(), a.element_size()
+    ends = [((t.shape[1] - 1) * t.stride(1) + t.shape[2]) * size for t in (a, b)]
+    at = (b.data_ptr() - a.data_ptr()) % (st * size) if st else 0
+    return b.stride(0) != st or at < ends[0] or at + ends[1] > st * size
+
+
 def call_on(device: torch.device, name: str, *args) -> int:
     """``call`` with the device's current torch stream as the last argument, the device made current
     for the launch where it is not."""

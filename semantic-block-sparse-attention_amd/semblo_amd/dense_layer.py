@@ -13,6 +13,9 @@ With ``keep_blocks`` the layer also weighs the cache's blocks as it decodes, and
 more cuts it to the ``keep_blocks`` most attended ones (the first ``sink_blocks`` and the last ``recent_blocks`` always
 stay).  With ``rotary`` the layer rotates the queries and keys itself: the operator's q_pre and k_pre are then
 all it reads, and q_post and k_post may be any tensors.
+
+The layer counts its tokens on the host, so its calls cannot be captured in a HIP graph (they raise): a captured decode
+calls the cache itself, ``layer.cache.append`` and ``layer.cache.attend``.
 """
 from __future__ import annotations
 
@@ -58,6 +61,16 @@ class DenseCacheAttention:
             raise ValueError(f"{what} must hold {heads} heads of {self.head_dim} per token, got {list(x.shape)}")
         return x.view(t, heads, self.head_dim) if x.is_contiguous() else x.reshape(t, heads, self.head_dim)
 
+    def reset(self) -> None:
+        """Ends the request: the next call starts a new one (as a prompt of more than one token does by itself)."""
+        self.cache.reset()
+        self.tokens = 0
+
+    @staticmethod
+    def _not_captured() -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a dense layer counts its tokens on the host: capture its cache's append and attend instead")
+
     def _room(self, tokens: int) -> None:
         """Makes room for ``tokens`` more, by an eviction where the layer evicts."""
         if self.tokens + tokens <= self.cache.capacity:
@@ -75,8 +88,8 @@ class DenseCacheAttention:
         t = q.shape[0]
         if t > self.cache.capacity:
             raise RuntimeError(f"a prompt of {t} tokens passes the cache's room for {self.cache.capacity}")
-        self.cache.reset()
-        self.tokens = 0
+        self._not_captured()
+        self.reset()
         out = output.view(t, self.num_heads, self.head_dim)
         most = dense_launch_queries(self.num_kv_heads, self.num_heads // self.num_kv_heads)
         if k.stride() != v.stride():
@@ -93,6 +106,7 @@ class DenseCacheAttention:
     def extend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, output: torch.Tensor) -> torch.Tensor:
         """More tokens of the request (one, or several at once), over the cache: as ``prefill``."""
         t = q.shape[0]
+        self._not_captured()
         self._room(t)
         self.cache.append(k, v)
         self.tokens += t

@@ -238,9 +238,9 @@ class QuantizedKVCache:
                out: torch.Tensor | None = None):
         """Attention of the newest tokens (their K/V are in the cache already): ``q`` [T, Hq, D] bfloat16, rows to sequences as
         in ``append``; row i of a sequence's n sees its first length - n + i + 1 tokens, and gives 0 (and an LSE of
-        -inf) where there are none.  Hq / Hkv up to 16.  Rows of no sequence keep what ``out`` held.
+        -inf) where there are none.  Hq / Hkv up to 16.  Rows of no sequence keep what ``out`` held, and have no LSE.
         ``accumulate`` adds to ``weights`` the probabilities each block received, over the rows and the query heads
-        of its KV head.  ``max_rows``: a hint, the most rows of a sequence.  Returns out [T, Hq, D], or (out, lse
+        of its KV head.  ``max_rows``: a hint, the most rows of a sequence.  Rows times query heads stay below 2^24.  Returns out [T, Hq, D], or (out, lse
         [T, Hq] fp32, natural)."""
         q = self._rows(q, "q", None)
         tokens, hq, d = q.shape
@@ -251,8 +251,8 @@ class QuantizedKVCache:
         if out is None:
             out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(0) % 8 or \
-                out.stride(1) % 8 or out.data_ptr() % 16:
-            raise ValueError(f"out must be bfloat16 {list(q.shape)} with rows on 16 bytes")
+                out.stride(1) % 8 or out.data_ptr() % 16 or not all(out.stride()):
+            raise ValueError(f"out must be bfloat16 {list(q.shape)} with rows on 16 bytes, no two on the same")
         elif _lib.overlap(out, q):
             raise ValueError("out overlaps q")
         _lib.require_one_device(self.codes_k, q, out, offsets)

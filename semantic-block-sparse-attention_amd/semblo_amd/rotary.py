@@ -149,6 +149,7 @@ class RotaryEmbedding:
             raise ValueError(f"positions must be {[tokens] if self._axes is None else [self.num_axes, tokens]}, "
                              f"got {list(positions.shape)}")
         device = q.device
+        given = out_q is not None or out_k is not None
         if out_q is None:
             out_q = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
         else:
@@ -168,6 +169,8 @@ class RotaryEmbedding:
             kst, ksh, _ = k.stride()
             okst, oksh, _ = out_k.stride()
             kv = (k.data_ptr(), kst, ksh, out_k.data_ptr(), okst, oksh, k.shape[1])
+            if given and (_lib.rows_overlap(out_q, k) or _lib.rows_overlap(out_k, q) or _lib.rows_overlap(out_q, out_k)):
+                raise ValueError("an output overlaps the other one, or the other input")
         _lib.require_one_device(q, out_q, positions, k, out_k)
         turns, axes = self._tables(device)
         _lib.call_on(device, "sbsa_rotary", q.data_ptr(), qst, qsh, out_q.data_ptr(), ost, osh, q.shape[1], *kv,
@@ -177,8 +180,8 @@ class RotaryEmbedding:
         return out_q if k is None else (out_q, out_k)
 
     def _output(self, out: torch.Tensor, x: torch.Tensor, what: str) -> None:
-        if out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1:
-            raise ValueError(f"{what} must have its input's shape and type and a unit inner stride")
+        if out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1 or not all(out.stride()):
+            raise ValueError(f"{what} must have its input's shape and type, a unit inner stride and no stride of 0")
         if out.stride() != x.stride() or out.data_ptr() != x.data_ptr():
             if _lib.overlap(out, x):
                 raise ValueError(f"{what} overlaps its input without being it")

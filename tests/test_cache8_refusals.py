@@ -150,6 +150,17 @@ def test_wrong_embeddings_are_refused():
         rope(pos, buf[:2], out_q=buf[1:])
     with pytest.raises(RuntimeError, match="backward"):
         rope(pos, q.clone().requires_grad_())
+    k = torch.zeros(2, 3, 64, dtype=torch.bfloat16)
+    both = torch.zeros(2, 4 * 64, dtype=torch.bfloat16)         # a row's query head and three key heads
+    own_q, own_k = both[:, :64].view(2, 1, 64), both[:, 64:].view(2, 3, 64)
+    for call in (lambda: rope(pos, k[:, :1], k, out_q=k[:, :1]), lambda: rope(pos, own_q, own_k, out_k=both[:, :192].view(2, 3, 64)),
+                 lambda: rope(pos, q, q, out_q=own_q, out_k=own_q), lambda: rope(pos, own_k, q, out_q=own_k, out_k=own_k[:, 2:])):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+    with pytest.raises(ValueError, match="stride of 0"):
+        rope(pos, q, out_q=q[:1].clone().expand(2, 1, 64))
+    with pytest.raises(RuntimeError):                           # in place in one buffer: only the device is wrong here
+        rope(pos, own_q, own_k, out_q=own_q, out_k=own_k)
 
 
 def test_frequencies_and_axes():

@@ -112,7 +112,7 @@ def test_append_holds_the_same_however_the_rows_are_split(fmt, d):
     whole.append(k, v, offsets=_offsets(rows))
     assert whole.lengths[:, 0].tolist() == rows
     first = _offsets(rows).tolist()
-    for cuts, hint in (([1, 1, 1, 1], 1), ([37, 9, 64, 65], 7), ([149, 5, 63, 130], None)):
+    for cuts, hint in (([1, 1, 1, 1], 1), ([37, 9, 64, 65], 7), ([149, 5, 63, 130], None), ([149, 5, 63, 200], 1)):
         parts = _cache(4, 2, d, 320, fmt)
         at = [0] * 4
         while at != rows:
@@ -354,6 +354,48 @@ def test_places_outside_the_room_are_read_inside_it():
     torch.cuda.synchronize()
 
 
+def test_attend_with_a_negative_scale_and_a_scale_of_zero():
+    d = 128
+    cache = _cache(1, 2, d, 256, "e4m3")
+    cache.append(_rows(250, 2, d, 60), _rows(250, 2, d, 61))
+    for n in (2, 70):
+        q = _rows(n, 4, d, 62)
+        for scale in (-0.09, 0.0):
+            out, lse = cache.attend(q, sm_scale=scale, return_lse=True)
+            want, want_lse, _, tol, ltol = attention(cache, q, [n], sm_scale=scale)
+            within(out, want, tol, "out")
+            within(lse, want_lse, ltol, "lse")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_attend_of_many_rows_before_a_block_that_is_not_finite(fmt):
+    d = 128
+    cache = _cache(1, 1, d, 512, fmt)
+    k, v = _rows(400, 1, d, 63), _rows(400, 1, d, 64)
+    v[350, 0, 3] = float("inf")
+    cache.append(k, v)
+    q = _rows(120, 2, d, 65)
+    out, lse = cache.attend(q, return_lse=True)            # rows 0 .. 39 end before the block of rows 320 .. 383
+    assert torch.isfinite(lse).all()
+    assert torch.isfinite(out[:40]).all() and out[40:].isnan().all()
+    cache.append(k[:0], v[:0], start=torch.tensor([320], dtype=torch.int32, device="cuda"))
+    want, _, _, tol, _ = attention(cache, q[:40], [40])
+    within(out[:40], want, tol, "rows before")
+
+
+def test_offsets_that_do_not_ascend_stay_inside_the_tensors():
+    cache = _cache(3, 2, 128, 2048, "e4m3")
+    cache.append(_rows(3 * 1500, 2, 128, 66), _rows(3 * 1500, 2, 128, 67))
+    q = _rows(90, 4, 128, 68)
+    for bad in ([0, 80, 10, 90], [90, 40, 0, 90], [-5, 3, 1000, 90], [0, 2 ** 31 - 1, -2 ** 31, 7]):
+        offsets = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        for hint in (1, 90):
+            cache.attend(q, offsets=offsets, max_rows=hint, accumulate=True)
+            cache.append(q[:, :2], q[:, 2:], offsets=offsets, max_rows=hint)
+    torch.cuda.synchronize()
+    assert int(cache.lengths.max()) <= 2048
+
+
 # -- eviction -------------------------------------------------------------------------------
 
 
@@ -511,7 +553,7 @@ def test_wrong_tensors_are_refused():
                  lambda: cache.append(k, k, start=torch.zeros(2, dtype=torch.int32))):
         with pytest.raises(RuntimeError):
             call()
-    for call in (lambda: cache.attend(q, out=q), lambda: cache.attend(q, offsets=_offsets([4])),
+    for call in (lambda: cache.attend(q, out=q), lambda: cache.attend(q, out=torch.empty_like(q[:1]).expand(4, 4, 128)), lambda: cache.attend(q, offsets=_offsets([4])),
                  lambda: cache.attend(q, offsets=_offsets([2, 2]).long()), lambda: cache.append(k[:3], k[:3]),
                  lambda: cache.attend(q, out=torch.empty(4, 4, 129, dtype=q.dtype, device="cuda")[..., 1:])):
         with pytest.raises(ValueError):

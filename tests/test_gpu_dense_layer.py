@@ -97,6 +97,28 @@ def test_extend_goes_on_with_several_tokens():
         layer.extend(q[:70], k[:70], v[:70], out[:70])
 
 
+def test_a_request_of_one_token_and_a_capture():
+    d, hq, hkv = 128, 4, 2
+    layer = _layer("test.dense.one", d, hq, hkv, capacity=128)
+    from semblo_amd.attention_op import sparse_attention_op
+    empty = torch.empty(0, device="cuda")
+    for request in range(2):
+        layer.reset()
+        for step in range(3):
+            q, k, v = (_rows(1, h, d, 9 * request + 3 * step + i) for i, h in enumerate((hq, hkv, hkv)))
+            out = torch.empty(1, hq * d, dtype=torch.bfloat16, device="cuda")
+            sparse_attention_op(empty, empty, q, k, v, q, k, out, "test.dense.one")
+            assert layer.tokens == step + 1 and layer.cache.lengths.unique().tolist() == [step + 1]
+        want, _, _, tol, _ = attention(layer.cache, q, [1])
+        within(out.view(1, hq, d), want, tol, f"request {request}")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.cache.append(k, v)
+        with pytest.raises(RuntimeError, match="counts its tokens"):
+            layer.extend(q, k, v, out)
+    assert layer.tokens == 3
+
+
 def test_layers_of_both_kinds_share_the_operator():
     from semblo_amd.attention_op import registered_layer
     from semblo_amd.config import SembloRuntimeConfig

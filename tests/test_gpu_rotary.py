@@ -65,6 +65,17 @@ def test_matches_the_rotation(d, r, t, hq, hkv, interleaved):
         assert torch.equal(got[..., r:], x[..., r:])
 
 
+def test_rotates_in_place_in_one_buffer_of_queries_and_keys():
+    from semblo_amd.rotary import RotaryEmbedding
+    rotary = RotaryEmbedding(128, rotary_dim=64)
+    both = _rows(40, 6, 128, 3).reshape(40, -1).contiguous()
+    q, k = both[:, :512].view(40, 4, 128), both[:, 512:].view(40, 2, 128)
+    pos = torch.arange(40, device="cuda") + 70
+    want = rotary(pos, q, k)
+    rotary(pos, q, k, out_q=q, out_k=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
 @pytest.mark.parametrize("first", [0, -5000, 2 ** 20 - 3, 2 ** 31 - 2, 2 ** 40 + 12345])
 @pytest.mark.parametrize("scaling", [None, dict(kind="linear", factor=4.0), dict(kind="ntk", factor=8.0),
                                      dict(kind="yarn", factor=4.0, original_length=32768),
