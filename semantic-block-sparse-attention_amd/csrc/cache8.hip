@@ -731,7 +731,8 @@ __global__ __launch_bounds__(256, 2) void attend_keys_kernel(AttendArgs a) {
   using W = WaveRows<D, FMT, R>;
   constexpr int TILE = W::NT * W::NI * 64;          // floats of a wave's O
   constexpr int PIECES = D / W::SEG * 2;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem_keys[];
+  constexpr int LEFT = R * D > 4096 ? 2 : 4;        // results that the last step joins
+  __shared__ __attribute__((aligned(16))) unsigned char smem_keys[LEFT * TILE * sizeof(float)];
   float* fold = reinterpret_cast<float*>(smem_keys);      // after the keys
   u32x4_t* sq = reinterpret_cast<u32x4_t*>(smem_keys);    // before
   __shared__ float sm[4 * 64], sl[4 * 64];
@@ -823,7 +824,6 @@ __global__ __launch_bounds__(256, 2) void attend_keys_kernel(AttendArgs a) {
   w.total();
   // The waves' results joined.  Where all four do not fit LDS twice on a compute unit (32 rows of 256 dims),
   // the odd waves' go into the even ones' first.
-  constexpr int LEFT = R * D > 4096 ? 2 : 4;        // results that the last step joins
   auto leave = [&](int at) {
 #pragma unroll
     for (int t = 0; t < W::NT; ++t)
@@ -1535,12 +1535,16 @@ AttendPlan plan_attend(const sbsa_cache8* c, int num_q_heads, int64_t tokens, in
   p.tile_queries = p.tile_rows / g;
   const int64_t tiles = ragged ? tokens / p.tile_queries + c->num_seqs
                                : (uniform + p.tile_queries - 1) / p.tile_queries * c->num_seqs;
-  // The keys are shared out until there are two grid blocks for each of the card's 256 compute units; a
-  // tile of few rows or of few keys stays whole, which saves the join.
+  // The keys are shared out until there are two grid blocks for each of the card's 256 compute units.  (One token at
+  // 131272 keys: 512 shares 60.7 us, 768 67, 1024 65, 1536 70.)  For tiles of 128 rows there are 1024 where the tiles alone
+  // are 512 and more, or their last ones run alone: an 8192-token chunk at 16384 keys 885 us with 512 and 695 with 1024,
+  // but a 512-token one at 16000 keys 178 and 221.
+  // Up to 20 blocks, 5 to a wave, stay whole, which saves the join (one token, 18 blocks: 13.6 us so and 15.2
+  // shared; 29 blocks: 20.7 and 15.5).
   const int64_t heads = c->num_kv_heads;
   p.target = 0;
   const int64_t want = p.keys || tiles * heads < 512 ? 512 : 1024;
-  if (tiles * heads < want && c->num_blocks > 16) p.target = (int)(want / heads < 1 ? 1 : want / heads);
+  if (tiles * heads < want && c->num_blocks > 20) p.target = (int)(want / heads < 1 ? 1 : want / heads);
   p.slots = tiles + p.target;
   return p;
 }
@@ -1578,23 +1582,15 @@ int64_t weigh_blocks(const sbsa_cache8* c) {
   return (int64_t)((c->num_blocks + 255) / 256) * c->num_kv_heads * c->num_seqs;
 }
 
-template <int D, int FMT, int R>
-bool launch_keys(const AttendArgs& a, dim3 grid, hipStream_t stream) {
-  constexpr int lds = (R * D > 4096 ? 2 : 4) * R * D * (int)sizeof(float);
-  if (lds > 48 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(attend_keys_kernel<D, FMT, R>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
-    return false;
-  hipLaunchKernelGGL((attend_keys_kernel<D, FMT, R>), grid, dim3(256), lds, stream, a);
-  return true;
-}
-
 template <int D, int FMT>
-bool launch_attend(const AttendArgs& a, const AttendPlan& p, int accumulate, hipStream_t stream) {
+void launch_attend(const AttendArgs& a, const AttendPlan& p, int accumulate, hipStream_t stream) {
   const dim3 grid((unsigned)p.slots, (unsigned)a.c.num_kv_heads);
   if (!p.keys)
     hipLaunchKernelGGL((attend_rows_kernel<D, FMT>), grid, dim3(256), 0, stream, a);
-  else if (!(p.tile_rows == 16 ? launch_keys<D, FMT, 16>(a, grid, stream) : launch_keys<D, FMT, 32>(a, grid, stream)))
-    return false;
+  else if (p.tile_rows == 16)
+    hipLaunchKernelGGL((attend_keys_kernel<D, FMT, 16>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attend_keys_kernel<D, FMT, 32>), grid, dim3(256), 0, stream, a);
   if (p.target) {
     const int64_t join = join_blocks(&a.c, a.tokens, a.hq), weigh = a.part_w ? weigh_blocks(&a.c) : 0;
     if (few_shares(&a.c, a.tokens, a.hq))
@@ -1606,7 +1602,6 @@ bool launch_attend(const AttendArgs& a, const AttendPlan& p, int accumulate, hip
     hipLaunchKernelGGL((weigh_kernel<D, FMT>),
                        dim3((unsigned)((a.c.num_blocks + 3) / 4), (unsigned)a.c.num_kv_heads, (unsigned)a.c.num_seqs),
                        dim3(256), 0, stream, a);
-  return true;
 }
 
 }  // namespace
@@ -1683,12 +1678,12 @@ extern "C" int sbsa_cache8_attend(const sbsa_cache8* cache, const void* q, int64
   a.tile_queries = p.tile_queries; a.tile_rows = p.tile_rows; a.slots = (int)p.slots; a.target = p.target;
   a.scale_log2 = sm_scale * LOG2E;
   const bool e4m3 = cache->format == SBSA_CACHE8_E4M3;
-  const bool ok = cache->head_dim == 128
-                      ? (e4m3 ? launch_attend<128, SBSA_CACHE8_E4M3>(a, p, accumulate, stream)
-                              : launch_attend<128, SBSA_CACHE8_INT8>(a, p, accumulate, stream))
-                      : (e4m3 ? launch_attend<256, SBSA_CACHE8_E4M3>(a, p, accumulate, stream)
-                              : launch_attend<256, SBSA_CACHE8_INT8>(a, p, accumulate, stream));
-  if (!ok) return SBSA_ERR_LAUNCH;
+  if (cache->head_dim == 128)
+    e4m3 ? launch_attend<128, SBSA_CACHE8_E4M3>(a, p, accumulate, stream)
+         : launch_attend<128, SBSA_CACHE8_INT8>(a, p, accumulate, stream);
+  else
+    e4m3 ? launch_attend<256, SBSA_CACHE8_E4M3>(a, p, accumulate, stream)
+         : launch_attend<256, SBSA_CACHE8_INT8>(a, p, accumulate, stream);
   SBSA_CHECK_LAUNCH();
   return SBSA_OK;
 }

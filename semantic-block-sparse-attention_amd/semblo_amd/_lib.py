@@ -129,6 +129,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+# The current device without torch.cuda's check that the GPU is initialised (a tensor of it is there)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 # The handle itself, without the Stream object around it (a tenth of the time), where torch has the call
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -155,6 +157,11 @@ def require_one_device(first: torch.Tensor, *others: torch.Tensor | None) -> Non
             raise RuntimeError(f"one call's tensors lie on {first.device} and {t.device}")
 
 
+def rows_like(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape, type and device (``empty_like`` takes half of ``empty``'s 2.2 us)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the address ranges of two tensors meet."""
     def span(t):
@@ -179,7 +186,7 @@ def rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 def call_on(device: torch.device, name: str, *args) -> int:
     """``call`` with the device's current torch stream as the last argument, the device made current
     for the launch where it is not."""
-    if device.type != "cuda" or device.index == torch.cuda.current_device():
+    if device.type != "cuda" or device.index == _CURRENT_DEVICE():
         rc = getattr(_LIB or load(), name)(*args, stream(device))
         if rc != 0:
             raise RuntimeError(f"{name} failed: {ERRORS.get(rc, rc)}")

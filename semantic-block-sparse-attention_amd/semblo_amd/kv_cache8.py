@@ -94,16 +94,18 @@ class CacheTables:
         if out is not self:
             if out.table.shape != self.table.shape:
                 raise ValueError(f"into holds tables {list(out.table.shape)}, these are {list(self.table.shape)}")
-            for name in self.__slots__:
-                a, b = getattr(self, name), getattr(out, name)
-                if a.data_ptr() != b.data_ptr() and _lib.overlap(a, b):
-                    raise ValueError(f"into's {name} overlaps the tables' own")
         s, h, n = self.table.shape
-        _lib.require_one_device(self.table, self.weights, self.lengths, self.open_block, out.table, out.weights,
-                                out.lengths, out.open_block)
-        _lib.call_on(self.table.device, "sbsa_cache8_evict", self.table.data_ptr(), self.weights.data_ptr(),
-                     self.lengths.data_ptr(), self.open_block.data_ptr(), out.table.data_ptr(), out.weights.data_ptr(),
-                     out.lengths.data_ptr(), out.open_block.data_ptr(), s, h, n, keep, sink, recent)
+        mine = (self.table, self.weights, self.lengths, self.open_block)
+        others = mine if out is self else (out.table, out.weights, out.lengths, out.open_block)
+        at, to = [t.data_ptr() for t in mine], [t.data_ptr() for t in others]
+        for a, b, name in zip(at, to, self.__slots__):      # (contiguous, of 4-byte elements)
+            if a != b and abs(a - b) < (s * h * n if name in ("table", "weights") else s * h) * 4:
+                raise ValueError(f"into's {name} overlaps the tables' own")
+        if out is self:
+            _lib.require_one_device(*mine)
+        else:
+            _lib.require_one_device(*mine, *others)
+        _lib.call_on(self.table.device, "sbsa_cache8_evict", *at, *to, s, h, n, keep, sink, recent)
         return out
 
 
@@ -249,7 +251,7 @@ class QuantizedKVCache:
         at, hint = self._spread(tokens, offsets, max_rows)
         accumulate = bool(accumulate)
         if out is None:
-            out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
+            out = _lib.rows_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(0) % 8 or \
                 out.stride(1) % 8 or out.data_ptr() % 16 or not all(out.stride()):
             raise ValueError(f"out must be bfloat16 {list(q.shape)} with rows on 16 bytes, no two on the same")

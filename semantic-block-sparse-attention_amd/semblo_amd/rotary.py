@@ -151,7 +151,7 @@ class RotaryEmbedding:
         device = q.device
         given = out_q is not None or out_k is not None
         if out_q is None:
-            out_q = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
+            out_q = _lib.rows_like(q)
         else:
             self._output(out_q, q, "out_q")
         qst, qsh, _ = q.stride()
@@ -163,7 +163,7 @@ class RotaryEmbedding:
         else:
             self._rows(k, "k", tokens)
             if out_k is None:
-                out_k = torch.empty(k.shape, dtype=torch.bfloat16, device=device)
+                out_k = _lib.rows_like(k)
             else:
                 self._output(out_k, k, "out_k")
             kst, ksh, _ = k.stride()
