@@ -380,7 +380,7 @@ struct AttendArgs {
   f32x2_t* part_ml;            // [Hkv][slots][tile rows]
   i32x4_t* where;                 // [tokens * Hq]: a row's first slot, its slots, its place in the tile
   f32x2_t* row_ml;             // [tokens * Hq], with 1 / l (accumulating)
-  f32x2_t* part_w;             // [tokens * Hq][N]: each block's sum of a row (few rows, accumulating)
+  f32x2_t* part_w;             // [tokens * Hq][N][steps of a block]: each one's sum of a row (few rows, accumulating)
   const int32_t* offsets;
   int64_t tokens, uniform;
   int hq, g, tile_queries, tile_rows, slots, target;
@@ -484,7 +484,6 @@ __device__ __forceinline__ void finish_row(const AttendArgs& a, int64_t row, flo
 template <int D, int FMT, int R>
 struct WaveRows {
   static constexpr int PARTS = 64 / R;          // lanes that share a row
-  static constexpr int MINE = KB / PARTS;       // a lane's keys of a block
   static constexpr int STEPS = R == 16 ? 1 : 2; // a block of keys is taken in this many steps (32 rows: registers)
   static constexpr int GROUPS = KB / R / STEPS; // products of R keys in a step
   static constexpr int SEG = 16 * PARTS;        // dims that one 16-byte load of every part covers
@@ -493,7 +492,7 @@ struct WaveRows {
   static constexpr float P_SCALE = 0x1p11f, SLACK = 4.f;
   typedef __attribute__((ext_vector_type(NI))) float acc_t;
   typedef u32x4_t kcodes_t[GROUPS][D / SEG];
-  static constexpr int KEYS = MINE / STEPS;     // a lane's keys of a step: 16
+  static constexpr int KEYS = KB / PARTS / STEPS;       // a lane's keys of a step: 16
   typedef u32x4_t vcodes_t[NT];
 
   acc_t o[NT];
@@ -529,32 +528,34 @@ struct WaveRows {
     return qrow ? *reinterpret_cast<const u32x4_t*>(qrow + j * SEG + (lane / R) * 16 + x * 8) : zero;
   }
 
-  // the key (of a block's 64) that row r of product g takes
+  // the key of a step's that row r of product g takes
   static __device__ __forceinline__ int key_of(int r, int g) {
     if constexpr (R == 16)
       return (r >> 2) * 16 + g * 4 + (r & 3);
     else
-      return ((r >> 2) & 1) * 32 + g * 16 + (r >> 3) * 4 + (r & 3);
+      return ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3);
   }
+  // a lane's first key (of the block's 64) of a step
+  static __device__ __forceinline__ int mine(int step, int lane) { return step * (KB / STEPS) + (lane / R) * KEYS; }
 
   // A block's codes through a buffer resource of its size: the address of a load is a scalar base, one lane
   // offset and a scalar or literal one.  (By pointers the compiler carries 64-bit lane addresses and spills.)
   static __device__ __forceinline__ void load_k(const uint8_t* kb, int step, int lane, kcodes_t& kc) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)kb, 0, KB * D, BUFFER_CONFIG);
     if constexpr (R * D > 4096) lane = lane_again();      // the offset made here: registers less to keep
-    const int off = key_of(lane % R, 0) * D + (lane / R) * 16;
+    const int off = (step * (KB / STEPS) + key_of(lane % R, 0)) * D + (lane / R) * 16;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
       for (int j = 0; j < D / SEG; ++j)
-        kc[g][j] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, key_of(0, step * GROUPS + g) * D + j * SEG, 0);
+        kc[g][j] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, key_of(0, g) * D + j * SEG, 0);
   }
   static __device__ __forceinline__ void load_v(const uint8_t* vb, int step, int lane, vcodes_t& vc) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)vb, 0, KB * D, BUFFER_CONFIG);
     if constexpr (R * D > 4096) lane = lane_again();
-    const int off = (lane % R) * KB + (lane / R) * MINE;
+    const int off = (lane % R) * KB + mine(step, lane);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) vc[t] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, t * R * KB + step * KEYS, 0);
+    for (int t = 0; t < NT; ++t) vc[t] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, t * R * KB, 0);
   }
 
   // scores of a step's keys, times ks; q(j, x) gives the rows' pieces
@@ -724,7 +725,7 @@ struct LaneRow {
 };
 
 // Few rows per sequence: a tile of R rows over one share of the keys, every fourth block of keys to each
-// wave, the waves joined through LDS.  The codes go from memory to the registers that the products read,
+// wave (with 32 rows every fourth half of one: few blocks come to a wave, and a quarter of them idles less), the waves joined through LDS.  The codes go from memory to the registers that the products read,
 // the next block's on their way while this one's are used; no barrier and no LDS traffic but the queries'.
 template <int D, int FMT, int R>
 __global__ __launch_bounds__(256, 2) void attend_keys_kernel(AttendArgs a) {
@@ -752,13 +753,14 @@ __global__ __launch_bounds__(256, 2) void attend_keys_kernel(AttendArgs a) {
   const int64_t row = (int64_t)sh.s * c.num_kv_heads + h, base = row * c.num_blocks;
   const uint8_t* codes_k = (const uint8_t*)c.codes_k + base * KB * D;
   const uint8_t* codes_v = (const uint8_t*)c.codes_v + base * KB * D;
-  const int first = sh.lo + wave;
-  const int count = sh.hi > first ? (sh.hi - first + 3) / 4 : 0;
+  constexpr int STRIDE = 4 / W::STEPS;
+  const int step = wave % W::STEPS, first = sh.lo + wave / W::STEPS;
+  const int count = sh.hi > first ? (sh.hi - first + STRIDE - 1) / STRIDE : 0;
   // the places and scales of the wave's next 64 blocks: fetched by a lane each, kept in LDS
   __shared__ int s_place[4 * 64];
   __shared__ float s_ks[4 * 64], s_vs[4 * 64];
   auto fetch = [&](int i0, auto&& then) {           // then: what goes on as soon as the places are there
-    const int b = first + 4 * (i0 + lane);
+    const int b = first + STRIDE * (i0 + lane);
     int place = 0;
     if (b < sh.hi) {
       place = (int)(place_of(c, row, b) - base);
@@ -780,46 +782,35 @@ __global__ __launch_bounds__(256, 2) void attend_keys_kernel(AttendArgs a) {
   if (count > 0) {
     fetch(0, [&] {
       const int64_t at = place_at(0);
-      W::load_k(codes_k + at, 0, lane, kc);
-      W::load_v(codes_v + at, 0, lane, vc);
+      W::load_k(codes_k + at, step, lane, kc);
+      W::load_v(codes_v + at, step, lane, vc);
     });
   }
   for (int i = wave; i < PIECES; i += 4) sq[i * 64 + lane] = W::query_piece(qrow, i >> 1, i & 1, lane);
   __syncthreads();                                  // the queries are in LDS
-  float sum_m = 0.f, sum = 0.f;                     // the block's sum so far, at reference maximum sum_m
+  const int mine = W::mine(step, lane);
   for (int i = 0; i < count; ++i) {
-    const int b = first + 4 * i;
+    const int b = first + STRIDE * i;
     const float ksi = uniform(s_ks[wave * 64 + (i & 63)]), vsi = uniform(s_vs[wave * 64 + (i & 63)]);
-    const int64_t here = place_at(i);
     if (((i + 1) & 63) == 0) fetch(i + 1, [] {});
-    const int64_t next = i + 1 < count ? place_at(i + 1) : 0;
-#pragma unroll
-    for (int step = 0; step < W::STEPS; ++step) {
-      // what is loaded next: this block's next step, or the next block's first
-      const bool more = step + 1 < W::STEPS || i + 1 < count;
-      const int64_t at = step + 1 < W::STEPS ? here : next;
-      const int then = (step + 1) % W::STEPS, mine = (lane / R) * W::MINE + step * W::KEYS;
-      typename W::acc_t sc[W::GROUPS];
-      const int own = R * D > 4096 ? lane_again() : lane;       // a reload from scratch would wait for every load
-      W::scores(kc, [&](int j, int x) { return sq[(2 * j + x) * 64 + own]; }, ksi, sc);
-      if (more) W::load_k(codes_k + at, then, lane, kc);
-      u32x4_t p[W::KEYS / 8];
-      const float part_sum = w.softmax(sc, vsi, r.vis - b * KB - mine, (b + 1) * KB <= r.vis_least, p);
-      if (a.part_w) {
-        // the block's share of each row's attention, for the blocks' weights
-        sum = step == 0 ? part_sum : sum * (sum_m == w.m ? 1.f : __builtin_amdgcn_exp2f(sum_m - w.m)) + part_sum;
-        sum_m = w.m;
-        if (step + 1 == W::STEPS) {
-          if constexpr (R == 16) sum += __shfl_xor(sum, 16, 64);
-          sum += __shfl_xor(sum, 32, 64);
-          if (r.there && lane < R)
-            a.part_w[(r.token * a.hq + r.head) * c.num_blocks + b] = f32x2_t{w.m, sum};
-        }
-      }
-      w.values(vc, p, sh.held - b * KB - mine, sh.held - b * KB >= KB);
-      if (more) W::load_v(codes_v + at, then, lane, vc);
-      asm volatile("" ::: "memory");                // the queries stay in LDS, not in registers
+    const bool more = i + 1 < count;
+    const int64_t next = more ? place_at(i + 1) : 0;
+    typename W::acc_t sc[W::GROUPS];
+    const int own = R * D > 4096 ? lane_again() : lane;         // a reload from scratch would wait for every load
+    W::scores(kc, [&](int j, int x) { return sq[(2 * j + x) * 64 + own]; }, ksi, sc);
+    if (more) W::load_k(codes_k + next, step, lane, kc);
+    u32x4_t p[W::KEYS / 8];
+    float sum = w.softmax(sc, vsi, r.vis - b * KB - mine, (b + 1) * KB <= r.vis_least, p);
+    if (a.part_w) {
+      // what the row gives to the block's keys here, for the blocks' weights
+      if constexpr (R == 16) sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if (r.there && lane < R)
+        a.part_w[((r.token * a.hq + r.head) * c.num_blocks + b) * W::STEPS + step] = f32x2_t{w.m, sum};
     }
+    w.values(vc, p, sh.held - b * KB - mine, sh.held - b * KB >= KB);
+    if (more) W::load_v(codes_v + next, step, lane, vc);
+    asm volatile("" ::: "memory");                  // the queries stay in LDS, not in registers
   }
   w.total();
   // The waves' results joined.  Where all four do not fit LDS twice on a compute unit (32 rows of 256 dims),
@@ -1000,7 +991,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
   // per-lane places in the tiles: the keys' row of each half (its swizzle does not depend on the half: bits 0, 1, 2
   // and 5 of the row), the values' row of a 32-dim tile
   using W = WaveRows<D, FMT, 32>;
-  const int krow = W::key_of(lane % 32, 0);
+  const int lane_row = lane % 32, krow = ((lane_row >> 2) & 1) * 32 + (lane_row >> 3) * 4 + (lane_row & 3);
   const uint32_t klane = krow * D + ((part ^ T::key_swizzle(krow)) * 16);
   const uint32_t vlane = (lane % 32) * KB + (((2 * part) ^ ((lane >> 1) & 3)) * 16);
 
@@ -1271,8 +1262,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks
     for (int x = 0; x < 32 && r0 + x < (int64_t)n * a.g; ++x) {
       const int qi = (int)((r0 + x) / a.g);
       if (b * KB >= held - n + qi + 1 || b >= c.num_blocks) continue;      // the row does not see the block
-      const f32x2_t w = a.part_w[((row0 + qi) * a.hq + h * a.g + (r0 + x) % a.g) * c.num_blocks + b], all = row_ml[x];
-      sum += w.y == 0.f ? 0.f : w.y * __builtin_amdgcn_exp2f(w.x - all.x) * all.y;
+      const int steps = a.tile_rows / 16;
+      const f32x2_t* w = a.part_w + (((row0 + qi) * a.hq + h * a.g + (r0 + x) % a.g) * c.num_blocks + b) * steps;
+      const f32x2_t all = row_ml[x];
+      for (int y = 0; y < steps; ++y) sum += w[y].y == 0.f ? 0.f : w[y].y * __builtin_amdgcn_exp2f(w[y].x - all.x) * all.y;
     }
   }
   if (n > 0 && b < c.num_blocks && b * KB < held) c.weights[sh * c.num_blocks + b] += sum;
@@ -1331,7 +1324,7 @@ __global__ __launch_bounds__(256) void weigh_kernel(AttendArgs a) {
       for (int g = 0; g < W::GROUPS; ++g)
 #pragma unroll
         for (int i = 0; i < W::NI; ++i)
-          sum += (lane / 32) * W::MINE + step * W::KEYS + g * W::NI + i < x.seen
+          sum += W::mine(step, lane) + g * W::NI + i < x.seen
                      ? __builtin_amdgcn_exp2f(fminf(sc[g][i], FLT_MOST) - x.all.x) * x.all.y
                      : 0.f;
     }
@@ -1563,7 +1556,7 @@ AttendSpace attend_space(const AttendPlan& p, const sbsa_cache8* c, int64_t toke
   x.part = 2 * shares;
   x.where = p.target ? 4 * rows : 0;
   x.row = accumulate && !(p.keys && p.target) ? (2 * rows + 3) / 4 * 4 : 0;
-  x.w = accumulate && p.keys && p.target ? 2 * rows * c->num_blocks : 0;
+  x.w = accumulate && p.keys && p.target ? 2 * rows * c->num_blocks * (p.tile_rows / 16) : 0;
   return x;
 }
 
