@@ -1357,22 +1357,24 @@ struct EvictArgs {
 };
 
 constexpr int EVICT_THREADS = 1024;
+constexpr int EVICT_MOST = SBSA_CACHE8_MAX_BLOCKS / EVICT_THREADS;      // blocks of a thread
 
-// One (sequence, head): tables into LDS whole (the outputs may be the inputs); the weight of the last block that
-// stays by three histograms over its bits (not negative, so their order is that of the numbers), 11, 11
-// and 9 of them; then each wave counts its run of blocks, and writes it in order behind those before.
+// One (sequence, head).  The tables come through LDS into registers (the outputs may be the inputs), a run of 4 to 16 blocks to
+// a thread, so that counts need one scan and no ballots; the weight of the last block that stays by three histograms over
+// its bits (not negative, so their order is that of the numbers), 11, 11 and 9 of them; then the blocks in their new order
+// through LDS and out.
 __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
   constexpr int BINS = 2048, WAVES = EVICT_THREADS / 64;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_evict[];
+  const int room = a.num_blocks, room4 = (room + 3) / 4 * 4;
   int32_t* tab = reinterpret_cast<int32_t*>(smem_evict);
-  uint32_t* bits = reinterpret_cast<uint32_t*>(tab + a.num_blocks);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(tab + room4);
   __shared__ int hist[BINS];
-  __shared__ int part[WAVES], part_eq[WAVES];
+  __shared__ int part[WAVES];
   __shared__ int s_bin[2];
-  const int64_t sh = blockIdx.x, base = sh * a.num_blocks;
+  const int64_t sh = blockIdx.x, base = sh * room;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int room = a.num_blocks;
   int len = a.lengths[sh];
   len = len < 0 ? 0 : (len < room * KB ? len : room * KB);
   const int open = a.open_block[sh];
@@ -1381,13 +1383,29 @@ __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
     tab[i] = a.table[base + i];
     bits[i] = __float_as_uint(a.weights[base + i]);
   }
+  hist[tid] = 0;
+  hist[tid + EVICT_THREADS] = 0;
+  __syncthreads();
   const bool cuts = n > a.keep;
   const int stay = cuts ? a.keep : n;
-  const int mid0 = a.sink, mid1 = n - a.recent;       // used where the sequence is cut
-  auto key = [&](int i) -> uint32_t {
-    const uint32_t b = bits[i];
-    return __uint_as_float(b) > 0.f ? b : 0u;
-  };
+  const int mid0 = a.sink, mid1 = cuts ? n - a.recent : 0;      // the blocks of which some go
+  // this thread's blocks, and the keys of those in the middle (0 for a weight that is not above 0)
+  const int per = (room + 4 * EVICT_THREADS - 1) / (4 * EVICT_THREADS) * 4, b0 = tid * per;
+  u32x4_t t[EVICT_MOST / 4], w[EVICT_MOST / 4], k[EVICT_MOST / 4];
+#pragma unroll
+  for (int x = 0; x < EVICT_MOST; x += 4) {
+    if (x >= per) continue;
+    const int at = b0 + x < room4 ? b0 + x : 0;
+    t[x / 4] = *reinterpret_cast<const u32x4_t*>(tab + at);
+    w[x / 4] = *reinterpret_cast<const u32x4_t*>(bits + at);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int b = b0 + x + y;
+      k[x / 4][y] = b >= mid0 && b < mid1 && __uint_as_float(w[x / 4][y]) > 0.f ? w[x / 4][y] : 0u;
+    }
+  }
+  // a sum over the threads before this one, and the wave's last lane's sum left for the others
+  auto before_wave = [&] { return wave_sum_i32_dpp(lane < wave ? part[lane & (WAVES - 1)] : 0); };
   // bound: the key of the last of the heaviest `wanted` of the middle; above: how many are heavier
   uint32_t bound = 0;
   int above = 0;
@@ -1396,24 +1414,24 @@ __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
     constexpr int SHIFT[3] = {20, 9, 0}, WIDTH[3] = {11, 11, 9};
 #pragma unroll
     for (int round = 0; round < 3; ++round) {
-      hist[tid] = 0;
-      hist[tid + EVICT_THREADS] = 0;
-      __syncthreads();
-      for (int i = mid0 + tid; i < mid1; i += EVICT_THREADS) {
-        const uint32_t k = key(i), digit = (k >> SHIFT[round]) & ((1u << WIDTH[round]) - 1);
+#pragma unroll
+      for (int x = 0; x < EVICT_MOST; ++x) {
+        if (x >= per) continue;
+        const uint32_t key = k[x / 4][x % 4], digit = (key >> SHIFT[round]) & ((1u << WIDTH[round]) - 1);
         // (digit 0 need not be counted: it is where the bound lies if it is in no other bin)
-        if (digit && (round == 0 || k >> (SHIFT[round] + WIDTH[round]) == bound >> (SHIFT[round] + WIDTH[round])))
+        if (digit && (round == 0 || key >> (SHIFT[round] + WIDTH[round]) == bound >> (SHIFT[round] + WIDTH[round])))
           atomicAdd(&hist[digit], 1);
       }
       __syncthreads();
       // keys in bins above this thread's pair, from the top: threads in reverse order
       const int hi = BINS - 1 - 2 * tid;
       const int h1 = hist[hi], h0 = hist[hi - 1];
-      const int incl = wave_incl_scan(h1 + h0);
+      hist[hi] = 0;
+      hist[hi - 1] = 0;
+      const int incl = wave_incl_scan_dpp(h1 + h0);
       if (lane == 63) part[wave] = incl;
       __syncthreads();
-      int before = above + incl - h1 - h0;
-      for (int i = 0; i < wave; ++i) before += part[i];
+      const int before = above + incl - h1 - h0 + before_wave();
       if (before < wanted && before + h1 >= wanted) {
         s_bin[0] = hi;
         s_bin[1] = before;
@@ -1428,55 +1446,47 @@ __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
   } else if (cuts) {
     bound = 0xffffffffu;                              // none of the middle stays
   }
-  const int ties = wanted - above;                    // of those at the bound, the first that stay
-  __syncthreads();
-  // this wave's run of blocks: how many stay for sure, and how many are at the bound
-  const int run = (room + WAVES * 64 - 1) / (WAVES * 64) * 64;
-  const int i0 = wave * run, i1 = min(i0 + run, room);
-  auto sure = [&](int i, bool& at_bound) {
-    at_bound = false;
-    if (i >= n) return false;
-    if (!cuts || i < mid0 || i >= mid1) return true;
-    const uint32_t k = key(i);
-    at_bound = k == bound;
-    return k > bound;
+  const int ties = wanted - above > 0 ? wanted - above : 0;     // of those at the bound, the first that stay
+  auto look = [&](int x, bool& sure, bool& tied) {
+    const int b = b0 + x;
+    const bool middle = b >= mid0 && b < mid1;
+    sure = b < n && (!middle || k[x / 4][x % 4] > bound);
+    tied = middle && k[x / 4][x % 4] == bound;
   };
-  int kept = 0, eq = 0;
-  for (int i = i0; i < i1; i += 64) {
-    bool at_bound = false;
-    const bool yes = i + lane < i1 && sure(i + lane, at_bound);
-    kept += __popcll(__ballot(yes));
-    eq += __popcll(__ballot(i + lane < i1 && at_bound));
+  // how many stay for sure (in the upper 16 bits) and how many are at the bound: at most 16384 each
+  int mine = 0;
+#pragma unroll
+  for (int x = 0; x < EVICT_MOST; ++x) {
+    if (x >= per) continue;
+    bool sure, tied;
+    look(x, sure, tied);
+    mine += (sure ? 1 << 16 : 0) + (tied ? 1 : 0);
   }
-  if (lane == 0) {
-    part[wave] = kept;
-    part_eq[wave] = eq;
-  }
-  __syncthreads();
-  int at = 0, seen = 0;
-  for (int w = 0; w < wave; ++w) {
-    at += part[w];
-    seen += part_eq[w];
-  }
-  at += min(seen, max(ties, 0));                      // of the ties before, those that stay
-  const unsigned long long below = (1ull << lane) - 1;
-  for (int i = i0; i < i1; i += 64) {
-    const int b = i + lane;
-    bool at_bound = false;
-    bool here = b < i1 && sure(b, at_bound);
-    at_bound = at_bound && b < i1;
-    const unsigned long long tied = __ballot(at_bound);
-    here = here || (at_bound && seen + __popcll(tied & below) < ties);
-    const unsigned long long all = __ballot(here);
-    const int before = at + __popcll(all & below);    // blocks that stay before this one
-    if (b < i1) {
-      const int to = here ? before : (b < n ? stay + b - before : b);
-      a.table_out[base + to] = tab[b];
-      a.weights_out[base + to] = here ? __uint_as_float(bits[b]) : 0.f;
+  const int incl = wave_incl_scan_dpp(mine);
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();                                    // and every thread has its blocks from LDS
+  const int before = before_wave() + incl - mine;
+  int seen = before & 0xffff, at = (before >> 16) + (seen < ties ? seen : ties);
+#pragma unroll
+  for (int x = 0; x < EVICT_MOST; ++x) {
+    if (x >= per) continue;
+    const int b = b0 + x;
+    bool sure, tied;
+    look(x, sure, tied);
+    const bool here = sure || (tied && seen < ties);
+    if (b < room) {
+      const int to = here ? at : (b < n ? stay + b - at : b);
+      tab[to] = (int32_t)t[x / 4][x % 4];
+      bits[to] = here ? w[x / 4][x % 4] : 0u;
       if (b == open) a.open_out[sh] = here ? to : -1;
     }
-    at += __popcll(all);
-    seen += __popcll(tied);
+    at += here;
+    seen += tied;
+  }
+  __syncthreads();
+  for (int i = tid; i < room; i += EVICT_THREADS) {
+    a.table_out[base + i] = tab[i];
+    a.weights_out[base + i] = __uint_as_float(bits[i]);
   }
   if (tid == 0) {
     a.lengths_out[sh] = len - (n - stay) * KB;
@@ -1692,7 +1702,7 @@ extern "C" int sbsa_cache8_evict(const int32_t* table, const float* weights, con
   if (num_blocks > SBSA_CACHE8_MAX_BLOCKS || num_seqs > 65535 || num_kv_heads > 65535) return SBSA_ERR_UNSUPPORTED;
   const EvictArgs a{table, weights, lengths, open_block, table_out, weights_out, lengths_out, open_block_out,
                     num_blocks, keep, sink, recent};
-  const size_t lds = (size_t)num_blocks * 8;
+  const size_t lds = (size_t)(num_blocks + 3) / 4 * 32;
   if (lds > 48 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(evict_kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return SBSA_ERR_LAUNCH;

@@ -380,8 +380,10 @@ __forceinline__ VC mfma_f16(V8 a, V8 b, VC c) {
 }
 }  // namespace emu
 #define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, hi) emu::cvt_pk_f16_fp8((w), (s), (hi))
-#define __builtin_amdgcn_mbcnt_lo(m, x) (0u)
-#define __builtin_amdgcn_mbcnt_hi(m, x) ((unsigned)emu::lane())
+#define __builtin_amdgcn_mbcnt_lo(m, x) \
+  ((unsigned)(x) + (unsigned)__builtin_popcount((unsigned)(m) & (emu::lane() < 32 ? (1u << emu::lane()) - 1u : ~0u)))
+#define __builtin_amdgcn_mbcnt_hi(m, x) \
+  ((unsigned)(x) + (unsigned)__builtin_popcount((unsigned)(m) & (emu::lane() < 32 ? 0u : (1u << (emu::lane() - 32)) - 1u)))
 #define __builtin_amdgcn_permlane16_swap(a, b, f, c) emu::permlane16_swap((a), (b), (f), (c))
 #define __builtin_amdgcn_perm(a, b, sel) emu::perm((a), (b), (sel))
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) emu::mfma_f16<32>((a), (b), (c))
