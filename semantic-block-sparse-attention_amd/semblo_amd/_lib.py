@@ -158,8 +158,12 @@ def require_one_device(first: torch.Tensor, *others: torch.Tensor | None) -> Non
 
 
 def rows_like(x: torch.Tensor) -> torch.Tensor:
-    """A contiguous tensor of x's shape, type and device (``empty_like`` takes half of ``empty``'s 2.2 us)."""
-    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    """A contiguous tensor of x's shape [tokens, heads, dim], type and device (``empty`` takes 2.2 us of the host,
+    ``empty_like`` 1.2 and ``empty_strided`` 1.3)."""
+    if x.is_contiguous():
+        return torch.empty_like(x)
+    t, h, d = x.shape
+    return torch.empty_strided((t, h, d), (h * d, d, 1), dtype=x.dtype, device=x.device)
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
