@@ -182,7 +182,11 @@ typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 // bytes of it and those of a value column PASSES bytes of that; the values' turn through LDS only to leave in
 // whole rows of [dim][64].  No grid block moves a length that another may still read:
 // ONE: the call touches one block of a (sequence, head) at most, and the last of its two grid blocks (by a ticket) moves the
-// length on; otherwise append_end_kernel does (tickets of a long prompt's 1000 grid blocks on one address took as long as the rest).
+// length on; otherwise append_end_kernel does (tickets of a long prompt's 1000 grid blocks on one address took 11 us).
+//
+// Memory bounds a prompt: 32768 tokens of 4 heads of 256 dims read 134 MB and write 67 in 43 us, 4.7 TB/s, and the closing
+// kernel takes 4 more.  One token of 32 sequences takes 5.6 us: lengths, table, the open block's rows, one after another.
+// A rows' fence at the end (an L2 write-back by each grid block) had cost 70 us of 133.
 template <int D, int FMT, bool ONE>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int CH = D / 8;             // 16-byte pieces of a row
@@ -734,6 +738,10 @@ struct LaneRow {
 // Few rows per sequence: a tile of R rows over one share of the keys, every fourth block of keys to each
 // wave (with 32 rows every fourth half of one: few blocks come to a wave, and a quarter of them idles less), the waves joined through LDS.  The codes go from memory to the registers that the products read,
 // the next block's on their way while this one's are used; no barrier and no LDS traffic but the queries'.
+//
+// Memory bounds it: one token of 16 heads over 131272 keys of 4 heads of 256 dims (269 MB) takes 52 us, 5.2 TB/s, and
+// its join 5.6.  5 rows of each of 4 sequences up to 40009 keys (164 MB) take 40 us, 49 with whole blocks to a wave:
+// five halves come to each, and the start and the join of the waves show.
 template <int D, int FMT, int R>
 __global__ __launch_bounds__(256, 2) void attend_keys_kernel(AttendArgs a) {
   using W = WaveRows<D, FMT, R>;
@@ -894,6 +902,10 @@ __global__ __launch_bounds__(256, 2) void attend_keys_kernel(AttendArgs a) {
 // (half the LDS traffic of bf16 tiles, which would keep LDS as busy as the matrix cores) and each wave decodes what it reads;
 // a block of keys is taken in two halves of 32, so that two grid blocks fit a compute unit's registers and one's
 // softmax runs under the other's products.
+//
+// 2048 rows of 16 heads at 34777 keys of 4 heads of 256 dims take 1160 us, 980 TFLOP/s (a large bf16 product: 1220 to 1380).
+// What is left is vector work, the codes' decoding and the softmax: two waves of a SIMD do not cover it and the latency of
+// the LDS reads at every turn, and there are no registers for a third or for reads further ahead.
 //
 // LDS holds a block's tiles as 16-byte pieces, swizzled so that the 8 lanes of a read's cycle meet
 // different banks: piece c of key row r at c ^ key_swizzle(r), piece c of dim row d at c ^ (d / 2) % 4.  They come straight from
@@ -1158,7 +1170,7 @@ __device__ __forceinline__ bool shares_fit(const AttendArgs& a, const i32x4_t& w
 
 // The shares joined.  The first blocks of the grid each take 64 dims of a row, 16 threads to a share's 64 dims and every
 // 16th share to each (FEW: the 64 dims of 16 rows, every share of a row to its 16 threads); with part_w the others take 256 blocks of keys of a (sequence, head) and
-// add up what the rows left for each of them.
+// add up what the rows left for each of them.  Latency bounds it: 5.6 us for one token's 128 shares of 4 heads.
 template <int D, bool FEW>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -1279,7 +1291,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks
 }
 
 // The attention that each block receives: a wave holds a block of keys and goes over the rows that
-// see it, their sums known (lse); one addition per block, so no order of atomics enters.
+// see it, their sums known; one addition per block, so no order of atomics enters.  The keys form leaves the
+// sums to its join instead: for many rows, a float pair for each row and block would be more than the keys.  Decoding again for
+// every 32 rows bounds it: 130 rows at 65000 keys of 4 heads of 128 dims 86 us, 132 with the rows not loaded ahead.
 template <int D, int FMT>
 __global__ __launch_bounds__(256) void weigh_kernel(AttendArgs a) {
   using W = WaveRows<D, FMT, 32>;
@@ -1369,7 +1383,8 @@ constexpr int EVICT_MOST = SBSA_CACHE8_MAX_BLOCKS / EVICT_THREADS;      // block
 // One (sequence, head).  The tables come through LDS into registers (the outputs may be the inputs), a run of 4 to 16 blocks to
 // a thread, so that counts need one scan and no ballots; the weight of the last block that stays by three histograms over
 // its bits (not negative, so their order is that of the numbers), 11, 11 and 9 of them; then the blocks in their new order
-// through LDS and out.
+// through LDS and out.  Instructions and barriers bound it (one compute unit to a list): 128 lists of 8192 blocks take
+// 14 us, 17.6 with a ballot for every 64 blocks; 4 of 2304 7.2 us and 8.2.
 __global__ __launch_bounds__(EVICT_THREADS) void evict_kernel(EvictArgs a) {
   constexpr int BINS = 2048, WAVES = EVICT_THREADS / 64;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem_evict[];
@@ -1540,6 +1555,9 @@ AttendPlan plan_attend(const sbsa_cache8* c, int num_q_heads, int64_t tokens, in
   const int g = num_q_heads / c->num_kv_heads;
   const int64_t uniform = tokens / c->num_seqs;
   const int64_t most = ragged ? (max_rows < 1 || max_rows > tokens ? tokens : max_rows) : uniform;
+  // Up to 32 rows of a sequence to a KV head, the waves split the keys; with more they split the rows.  (20 rows of 4 sequences up
+  // to 40009 keys, D = 256: 47.8 us so, 53.5 in a tile of 128 rows; of 8 up to 16384, D = 128: 24.5 and 30.7.)  Up to 16
+  // rows, in tiles of 16: 41.7 us for 16 rows where 20 take 47.8.
   p.keys = most * g <= 32;
   p.tile_rows = !p.keys ? 128 : most * g <= 16 ? 16 : 32;
   p.tile_queries = p.tile_rows / g;

@@ -8,6 +8,9 @@
 // HEADS heads, every HEADS-th group of them to a thread: the sines of its pairs are made once for HEADS heads, and its
 // loads are all on their way before the first is used.  The work is a row of items over all threads, so
 // that no thread is left over whatever the head count and the rotated share.
+//
+// Memory bounds it: 32768 tokens of 16 + 4 heads of 256 dims (671 MB) take 145 us, 4.6 TB/s.  One token takes 3.2 us, which is
+// the chain of its loads (position, frequency, row).
 #include "sbsa_common.h"
 
 namespace {
@@ -137,7 +140,8 @@ bool launch_rotary(RotaryArgs a, int64_t tokens, int head_dim, bool in_place, in
   a.units = a.rot_units + (in_place ? 0 : (head_dim - a.rotary_dim) / VEC);
   const int64_t rows = tokens * a.units;
   if (rows * (a.hq + a.hkv) >= (1ll << 32) - 256) return false;
-  // a thread per head until there are threads for half of the card's 524288 places, then four heads to each
+  // a thread per head until there are threads for half of the card's 524288 places, then four heads to each (one token:
+  // 3.2 us with one, 4.2 with four; 3001 tokens of 10 heads 7.5 and 7.3; 32768 of 20 heads 293 and 149)
   if (rows * (a.hq + a.hkv) <= 262144)
     launch_heads<VEC, 1>(a, rows, interleaved, stream);
   else
@@ -173,6 +177,7 @@ extern "C" int sbsa_rotary(const void* q, int64_t q_st, int64_t q_sh, void* q_ou
            aligned(q_out, qo_st, qo_sh, vec) &&
            (num_kv_heads == 0 || (aligned(k, k_st, k_sh, vec) && aligned(k_out, ko_st, ko_sh, vec)));
   };
+  // pieces of 16 bytes where sizes and alignment allow them, else of 4 (32768 tokens: 149 us, 271 with 4), else single values
   const bool ok = fits(8)   ? launch_rotary<8>(a, tokens, head_dim, in_place, interleaved, stream)
                   : fits(2) ? launch_rotary<2>(a, tokens, head_dim, in_place, interleaved, stream)
                             : launch_rotary<1>(a, tokens, head_dim, in_place, interleaved, stream);
