@@ -16,7 +16,8 @@ one fp32 scale for its keys and one for its values: the largest magnitude over 4
 last block are kept in bf16 as well, and the block is quantised again whole whenever rows join it, so
 that what a cache holds does not depend on how its tokens were split into calls.
 
-Calls on one cache belong on one stream, or on streams that wait for one another.
+Calls on one cache belong on one stream, or on streams that wait for one another.  Its tensors are fixed when it is made:
+what they hold may be copied over, the attributes not be replaced.
 """
 from __future__ import annotations
 
@@ -149,6 +150,8 @@ class QuantizedKVCache:
         self.codes_k, self.codes_v, self.scales, self.tail, self.tables = codes_k, codes_v, scales, tail, tables
         self.fmt, self.device = fmt, codes_k.device
         self.num_seqs, self.num_kv_heads, self.num_blocks, self.head_dim = s, h, n, d
+        # what the kernels' struct points to stays alive, whatever becomes of the attributes
+        self._alive = (codes_k, codes_v, scales, tail, *(getattr(tables, name) for name in tables.__slots__))
         # the append's tickets, zero between calls, and its flag for rows that found no room
         self._counters = torch.zeros(s * h + 1, dtype=torch.int32, device=self.device)
         self._struct = _Cache8(
@@ -229,7 +232,7 @@ class QuantizedKVCache:
             raise ValueError(f"{tokens // self.num_seqs} rows of a sequence pass its room of {self.capacity}")
         if start is not None:
             _check(start, "start", (self.num_seqs,), torch.int32)
-        _lib.require_one_device(self.codes_k, k, v, offsets, start)
+        _lib.require_one_device(self._alive[0], k, v, offsets, start)
         kst, ksh, _ = k.stride()
         vst, vsh, _ = v.stride()
         _lib.call_on(self.device, "sbsa_cache8_append", self._ref, k.data_ptr(), kst, ksh, v.data_ptr(), vst, vsh, tokens,
@@ -257,7 +260,7 @@ class QuantizedKVCache:
             raise ValueError(f"out must be bfloat16 {list(q.shape)} with rows on 16 bytes, no two on the same")
         elif _lib.overlap(out, q):
             raise ValueError("out overlaps q")
-        _lib.require_one_device(self.codes_k, q, out, offsets)
+        _lib.require_one_device(self._alive[0], q, out, offsets)
         lse = torch.empty((tokens, hq), dtype=torch.float32, device=self.device) if return_lse else None
         # the workspace goes by sizes that the host knows; made anew by each call, so that captured graphs and streams have
         # their own

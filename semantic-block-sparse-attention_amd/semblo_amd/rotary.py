@@ -119,21 +119,24 @@ class RotaryEmbedding:
             section_axes(sections, rotary_dim // 2, sections_interleaved), dtype=torch.uint8)
         self._on: dict = {}
 
-    def _tables(self, device):
-        tables = self._on.get(device)
+    def _tables(self, q: torch.Tensor):
+        """(turns, axes, their addresses) on q's device."""
+        tables = self._on.get(q.get_device())
         if tables is None:
-            tables = (self._turns.to(device), None if self._axes is None else self._axes.to(device))
-            self._on[device] = tables
+            turns, axes = self._turns.to(q.device), None if self._axes is None else self._axes.to(q.device)
+            tables = self._on[q.get_device()] = (turns, axes, turns.data_ptr(), None if axes is None else axes.data_ptr())
         return tables
 
-    def _rows(self, x: torch.Tensor, what: str, tokens: int) -> None:
-        shape = x.shape
+    def _rows(self, x: torch.Tensor, what: str, tokens: int):
+        """(heads, token stride, head stride) of a call's queries or keys."""
+        shape, stride = x.shape, x.stride()
         if len(shape) != 3 or shape[0] != tokens or shape[2] != self.head_dim:
             raise ValueError(f"{what} must be [{tokens}, heads, {self.head_dim}], got {list(x.shape)}")
-        if x.dtype is not torch.bfloat16 or x.stride(2) != 1:
+        if x.dtype is not torch.bfloat16 or stride[2] != 1:
             raise ValueError(f"{what} must be bfloat16 with a unit inner stride")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("the rotary embedding has no backward pass: call it under torch.no_grad()")
+        return shape[1], stride[0], stride[1]
 
     def __call__(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None, *,
                  out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None, inverse: bool = False):
@@ -142,7 +145,7 @@ class RotaryEmbedding:
         negative ones too.  ``out_q``, ``out_k``: where to; the inputs themselves rotate in place.
         ``inverse`` rotates back (keys before the embedding from a cache's)."""
         tokens = q.shape[0]
-        self._rows(q, "q", tokens)
+        hq, qst, qsh = self._rows(q, "q", tokens)
         if positions.dtype is not torch.int64 and positions.dtype is not torch.int32:
             raise ValueError("positions must be int32 or int64")
         if positions.shape != ((tokens,) if self._axes is None else (self.num_axes, tokens)):
@@ -154,29 +157,27 @@ class RotaryEmbedding:
             out_q = _lib.rows_like(q)
         else:
             self._output(out_q, q, "out_q")
-        qst, qsh, _ = q.stride()
         ost, osh, _ = out_q.stride()
         if k is None:
             if out_k is not None:
                 raise ValueError("out_k without k")
             kv = (None, 0, 0, None, 0, 0, 0)
         else:
-            self._rows(k, "k", tokens)
+            hkv, kst, ksh = self._rows(k, "k", tokens)
             if out_k is None:
                 out_k = _lib.rows_like(k)
             else:
                 self._output(out_k, k, "out_k")
-            kst, ksh, _ = k.stride()
             okst, oksh, _ = out_k.stride()
-            kv = (k.data_ptr(), kst, ksh, out_k.data_ptr(), okst, oksh, k.shape[1])
+            kv = (k.data_ptr(), kst, ksh, out_k.data_ptr(), okst, oksh, hkv)
             if given and (_lib.rows_overlap(out_q, k) or _lib.rows_overlap(out_k, q) or _lib.rows_overlap(out_q, out_k)):
                 raise ValueError("an output overlaps the other one, or the other input")
         _lib.require_one_device(q, out_q, positions, k, out_k)
-        turns, axes = self._tables(device)
-        _lib.call_on(device, "sbsa_rotary", q.data_ptr(), qst, qsh, out_q.data_ptr(), ost, osh, q.shape[1], *kv,
+        _, axes, turns_at, axes_at = self._tables(q)
+        _lib.call_on(device, "sbsa_rotary", q.data_ptr(), qst, qsh, out_q.data_ptr(), ost, osh, hq, *kv,
                      positions.data_ptr(), positions.element_size(), positions.stride(0) if axes is not None else 0,
-                     positions.stride(-1), tokens, self.head_dim, self.rotary_dim, self.interleaved, turns.data_ptr(),
-                     None if axes is None else axes.data_ptr(), self.gain, inverse)
+                     positions.stride(-1), tokens, self.head_dim, self.rotary_dim, self.interleaved, turns_at,
+                     axes_at, self.gain, inverse)
         return out_q if k is None else (out_q, out_k)
 
     def _output(self, out: torch.Tensor, x: torch.Tensor, what: str) -> None:

@@ -396,6 +396,33 @@ def test_offsets_that_do_not_ascend_stay_inside_the_tensors():
     assert int(cache.lengths.max()) <= 2048
 
 
+def test_a_row_that_is_not_finite_leaves_the_others_alone():
+    d = 128
+    cache = _cache(1, 2, d, 512, "int8")
+    cache.append(_rows(450, 2, d, 70), _rows(450, 2, d, 71))
+    for n in (4, 9, 100):
+        q = _rows(n, 4, d, 72)
+        want, want_lse, _, tol, ltol = attention(cache, q, [n])
+        q[1, 2, 5], q[2, 0, 7] = float("nan"), float("inf")
+        out, lse = cache.attend(q, return_lse=True)
+        others = torch.ones(n, 4, dtype=torch.bool)
+        others[1, 2] = others[2, 0] = False
+        assert out[1, 2].isnan().all()
+        within(out.cpu()[others], want[others], tol[others], "out")
+        within(lse.cpu()[others], want_lse[others], ltol[others], "lse")
+
+
+def test_a_cache_keeps_its_tensors():
+    cache = _cache(1, 1, 128, 128, "e4m3")
+    k, v, q = _rows(100, 1, 128, 73), _rows(100, 1, 128, 74), _rows(1, 1, 128, 75)
+    cache.append(k, v)
+    want = cache.attend(q)
+    cache.codes_k = cache.codes_v = cache.scales = cache.tail = cache.tables = None
+    fill = [torch.full((1 << n,), 255, dtype=torch.uint8, device="cuda") for n in range(4, 20)]
+    assert torch.equal(cache.attend(q), want)
+    del fill
+
+
 # -- eviction -------------------------------------------------------------------------------
 
 
@@ -496,6 +523,33 @@ def test_a_captured_decode_replays_as_the_eager_one():
         if step % 23 == 0:
             torch.cuda.synchronize()
         assert torch.equal(out, eager), f"step {step}"
+        _same(_state(caches[0]), _state(caches[1]))
+
+
+def test_a_captured_ragged_call_follows_its_offsets():
+    """Prompts of several blocks and their attention captured together, replayed with other rows, counts and lengths."""
+    d, hkv, hq, seqs, tokens = 128, 2, 4, 3, 300
+    caches = [_cache(seqs, hkv, d, 1280, "e4m3", seed=6) for _ in range(2)]
+    k, v, q = _rows(tokens, hkv, d, 1), _rows(tokens, hkv, d, 2), _rows(tokens, hq, d, 3)
+    offsets, out = _offsets([100, 100, 100]), torch.zeros(tokens, hq, d, dtype=torch.bfloat16, device="cuda")
+    eager = out.clone()
+
+    def step(cache, to):
+        cache.append(k, v, offsets=offsets)
+        cache.attend(q, offsets=offsets, accumulate=True, out=to)
+    step(_cache(seqs, hkv, d, 1280, "e4m3"), out)          # warm up on another cache
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(caches[0], out)
+    for i, rows in enumerate(([100, 100, 100], [0, 299, 1], [7, 64, 200], [300, 0, 0], [1, 1, 1], [65, 0, 130])):
+        offsets.copy_(_offsets(rows))
+        for x, heads in ((k, hkv), (v, hkv), (q, hq)):
+            x.copy_(_rows(tokens, heads, d, 10 * i + heads))
+        graph.replay()
+        step(caches[1], eager)
+        if i % 2:
+            torch.cuda.synchronize()
+        assert torch.equal(out, eager), f"replay {i}"
         _same(_state(caches[0]), _state(caches[1]))
 
 
