@@ -4,6 +4,7 @@
 // A block is 64 tokens of one (sequence, KV head).  Keys lie [64][D], values [D][64]:
 // both are then the A operand of their product as they lie (S^T = K Q^T takes 8 dims of
 // a key per lane, O^T = V^T P^T 8 keys of a dim), and nothing is transposed in the attention.
+#include <algorithm>
 #include "sbsa_common.h"
 
 namespace {
@@ -1567,12 +1568,17 @@ AttendPlan plan_attend(const sbsa_cache8* c, int num_q_heads, int64_t tokens, in
   // 131272 keys: 512 shares 60.7 us, 768 67, 1024 65, 1536 70.)  For tiles of 128 rows there are 1024 where the tiles alone
   // are 512 and more, or their last ones run alone: an 8192-token chunk at 16384 keys 885 us with 512 and 695 with 1024,
   // but a 512-token one at 16000 keys 178 and 221.
-  // Up to 20 blocks, 5 to a wave, stay whole, which saves the join (one token, 18 blocks: 13.6 us so and 15.2
-  // shared; 29 blocks: 20.7 and 15.5).
+  // Up to 20 blocks of 128 dims or 10 of 256 stay whole, which saves the join (one token, 18 blocks of 128: 13.8 us so and
+  // 14.0 to 15.2 shared, 29: 20.7 and 15.5; 18 of 256: 18.6 and 14.6 to 15.8).
+  // No more shares than the room can fill: left-over grid blocks put the others two to a compute unit (57 blocks of 256
+  // dims: 19.4 us with them, 15.8 without).
   const int64_t heads = c->num_kv_heads;
   p.target = 0;
   const int64_t want = p.keys || tiles * heads < 512 ? 512 : 1024;
-  if (tiles * heads < want && c->num_blocks > 20) p.target = (int)(want / heads < 1 ? 1 : want / heads);
+  if (tiles * heads < want && c->num_blocks * c->head_dim > 20 * 128) {
+    const int64_t useful = tiles * ((c->num_blocks + 3) / 4);     // of 4 blocks, a share's least
+    p.target = (int)std::max<int64_t>(1, std::min(want / heads, useful));
+  }
   p.slots = tiles + p.target;
   return p;
 }
