@@ -187,7 +187,7 @@ typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 //
 // Memory bounds a prompt: 32768 tokens of 4 heads of 256 dims read 134 MB and write 67 in 43 us, 4.7 TB/s, and the closing
 // kernel takes 4 more.  One token of 32 sequences takes 5.6 us: lengths, table, the open block's rows, one after another.
-// A rows' fence at the end (an L2 write-back by each grid block) had cost 70 us of 133.
+// (A device fence at each grid block's end, an L2 write-back, had made a prompt's 64 us 133.)
 template <int D, int FMT, bool ONE>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int CH = D / 8;             // 16-byte pieces of a row
@@ -737,8 +737,9 @@ struct LaneRow {
 };
 
 // Few rows per sequence: a tile of R rows over one share of the keys, every fourth block of keys to each
-// wave (with 32 rows every fourth half of one: few blocks come to a wave, and a quarter of them idles less), the waves joined through LDS.  The codes go from memory to the registers that the products read,
-// the next block's on their way while this one's are used; no barrier and no LDS traffic but the queries'.
+// wave (with 32 rows every fourth half of one: few blocks come to a wave, and halves of them go round more evenly), the
+// waves joined through LDS.  The codes go from memory to the registers that the products read, the next block's on their
+// way while this one's are used; no barrier and no LDS traffic but the queries'.
 //
 // Memory bounds it: one token of 16 heads over 131272 keys of 4 heads of 256 dims (269 MB) takes 52 us, 5.2 TB/s, and
 // its join 5.6.  5 rows of each of 4 sequences up to 40009 keys (164 MB) take 40 us, 49 with whole blocks to a wave:
@@ -1170,8 +1171,9 @@ __device__ __forceinline__ bool shares_fit(const AttendArgs& a, const i32x4_t& w
 }
 
 // The shares joined.  The first blocks of the grid each take 64 dims of a row, 16 threads to a share's 64 dims and every
-// 16th share to each (FEW: the 64 dims of 16 rows, every share of a row to its 16 threads); with part_w the others take 256 blocks of keys of a (sequence, head) and
-// add up what the rows left for each of them.  Latency bounds it: 5.6 us for one token's 128 shares of 4 heads.
+// 16th share to each (FEW: the 64 dims of 16 rows, every share of a row to its 16 threads); with part_w the others take 256
+// blocks of keys of a (sequence, head) and add up what the rows left for each of them.  Latency bounds it: 5.6 us for one
+// token's 128 shares of 4 heads.
 template <int D, bool FEW>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int join_blocks) {
   const int tid = threadIdx.x, lane = tid & 63;

@@ -158,8 +158,8 @@ extern "C" int sbsa_rotary(const void* q, int64_t q_st, int64_t q_sh, void* q_ou
                            int interleaved, const uint64_t* turns, const uint8_t* axes, float gain, int inverse,
                            hipStream_t stream) {
   if (!turns || num_q_heads < 1 || num_kv_heads < 0 || tokens < 0 ||
-      (tokens > 0 && (!q || !q_out || !positions || (num_kv_heads > 0 && (!k || !k_out)))) || (pos_bytes != 4 && pos_bytes != 8) || rotary_dim < 2 ||
-      rotary_dim % 2 || rotary_dim > head_dim || !(gain > 0.f))
+      (tokens > 0 && (!q || !q_out || !positions || (num_kv_heads > 0 && (!k || !k_out)))) ||
+      (pos_bytes != 4 && pos_bytes != 8) || rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim || !(gain > 0.f))
     return SBSA_ERR_ARG;
   if (head_dim > 512 || tokens >= (1 << 24)) return SBSA_ERR_UNSUPPORTED;
   if (tokens == 0) return SBSA_OK;

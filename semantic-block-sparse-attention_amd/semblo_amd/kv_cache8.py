@@ -245,8 +245,8 @@ class QuantizedKVCache:
         in ``append``; row i of a sequence's n sees its first length - n + i + 1 tokens, and gives 0 (and an LSE of
         -inf) where there are none.  Hq / Hkv up to 16.  Rows of no sequence keep what ``out`` held, and have no LSE.
         ``accumulate`` adds to ``weights`` the probabilities each block received, over the rows and the query heads
-        of its KV head.  ``max_rows``: a hint, the most rows of a sequence.  Rows times query heads stay below 2^24.  Returns out [T, Hq, D], or (out, lse
-        [T, Hq] fp32, natural)."""
+        of its KV head.  ``max_rows``: a hint, the most rows of a sequence.  Rows times query heads stay below
+        2^24.  Returns out [T, Hq, D], or (out, lse [T, Hq] fp32, natural)."""
         q = self._rows(q, "q", None)
         tokens, hq, d = q.shape
         if hq < 1 or hq % self.num_kv_heads or hq // self.num_kv_heads > 16:

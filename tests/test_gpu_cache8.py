@@ -396,6 +396,24 @@ def test_offsets_that_do_not_ascend_stay_inside_the_tensors():
     assert int(cache.lengths.max()) <= 2048
 
 
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("blocks", [1, 10, 11, 20, 21, 33])
+def test_attend_whole_and_in_shares(blocks, d):
+    """Rooms on both sides of where a tile's keys are shared out."""
+    cache = _cache(2, 1, d, blocks * BLOCK, "int8")
+    lengths = [blocks * BLOCK, blocks * BLOCK - 37]
+    cache.append(_rows(sum(lengths), 1, d, 76), _rows(sum(lengths), 1, d, 77), offsets=_offsets(lengths))
+    for n in (1, 5, 17):
+        q = _rows(2 * n, 4, d, 78)
+        cache.weights.zero_()
+        out, lse = cache.attend(q, accumulate=True, return_lse=True)
+        want, want_lse, added, tol, ltol = attention(cache, q, [n, n])
+        within(out, want, tol, "out")
+        within(lse, want_lse, ltol, "lse")
+        # (sums of probabilities, each off by twice its row's bound, over fp32 sums of a block's 64 and a head's rows)
+        within(cache.weights, added, added * (2 * float(ltol.max()) + 2.0 ** -18) + 1e-30, "weights")
+
+
 def test_a_row_that_is_not_finite_leaves_the_others_alone():
     d = 128
     cache = _cache(1, 2, d, 512, "int8")
