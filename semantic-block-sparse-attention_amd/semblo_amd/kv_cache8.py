@@ -261,7 +261,8 @@ class QuantizedKVCache:
         elif _lib.overlap(out, q):
             raise ValueError("out overlaps q")
         _lib.require_one_device(self._alive[0], q, out, offsets)
-        lse = torch.empty((tokens, hq), dtype=torch.float32, device=self.device) if return_lse else None
+        # (empty_strided: as in rows_like)
+        lse = torch.empty_strided((tokens, hq), (hq, 1), dtype=torch.float32, device=self.device) if return_lse else None
         # the workspace goes by sizes that the host knows; made anew by each call, so that captured graphs and streams have
         # their own
         key = (hq, tokens, hint, at is None, accumulate)
@@ -271,7 +272,7 @@ class QuantizedKVCache:
                 self._needs.clear()
             need = self._needs[key] = _lib.query("sbsa_cache8_attend_workspace_bytes", self._ref, hq, tokens, hint,
                                                  at is not None, accumulate)
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        work = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=self.device) if need else None
         qst, qsh, _ = q.stride()
         ost, osh, _ = out.stride()
         _lib.call_on(self.device, "sbsa_cache8_attend", self._ref, q.data_ptr(), qst, qsh, hq, tokens, at, hint,
